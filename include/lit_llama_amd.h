@@ -645,6 +645,48 @@ int llj_gqa_decode(const void* in, int ld, int oq, int ok, int ov, int og, const
                    int ldf, float* part, int* count, int nsplit, void* y, int ldy, int M, int heads, int kv_heads, int dim, int vdim,
                    float scale, int sink, void* stream);
 
+/* ---------------------------------------------------------------- paged K / V caches in 4 bits
+ * No reference counterpart (lit_llama/pages.py, lit_llama/kv4.py). A page holds 16, 32, 64, 128 or 256 tokens of one sequence; table[slot][i]
+ * (rows of ldt ints) is the page of the slot's tokens i page .. (i + 1) page - 1, seen[slot] the tokens it holds, free_ids[0 .. *nfree) (room for
+ * cap) a stack of the pages nobody holds.
+ * extend: sequence b < B <= 4096 of a call, in slot[b] (slots <= 65536 of them), gets add[b] more tokens (add NULL: one each). Its new pages come
+ * off the stack, the first sequence's first, into its table. Rows m of the call, sequence by sequence: row0 (B + 1) the first of each, row_seq[m] the
+ * sequence, pos[m] the position, place[m] = page number * page + token in the page; rows behind the last, up to M: -1. chunk > 0: work
+ * items (first row, rows, sequence) of at most `chunk` rows, item0 (B + 1) the first of each sequence, those behind the last up to nwork
+ * zero. after (B): the sequences' tokens behind the call, left: the free pages; commit: both also into seen and nfree (without it the
+ * same call can be made again: the pages taken are still on the stack).
+ * release: the pages of B sequences onto the stack, their tokens 0 and their table entries -1.
+ * *status = 0, or the call was left undone (extend: without rows): 1 too few free pages; 2 a slot outside the tables or named twice, a negative
+ * count, more tokens than ldt pages, more rows than M or items than nwork, more pages than cap. fault (NULL: none) keeps all such bits. */
+int llj_pages_extend(const int* slot, const int* add, int B, int* seen, int slots, int* table, int ldt, const int* free_ids, int* nfree,
+                     int cap, int page, int commit, int* row0, int* item0, int* row_seq, int* pos, int* place, int M, int* work, int nwork,
+                     int chunk, int* after, int* left, int* status, int* fault, void* stream);
+int llj_pages_release(const int* slot, int B, int* seen, int slots, int* table, int ldt, int* free_ids, int* nfree, int cap, int page, int* status,
+                      int* fault, void* stream);
+/* The cache: pool [pages][kv_heads] blocks of llj_kv4_block_bytes (0: sizes not taken; dim, vdim 1 .. 256), one head's part of a page: [key codes
+ * page x Dp / 2 | value codes page x Vp / 2 | key pairs page x 4 | value pairs page x 4] bytes with Dp, Vp = 64, 128 or 256. Value i of a
+ * vector is 4 bits c_i of its word i / 8, bits 4 (i % 8) and up, and stands for c_i s + o, (s, o) its bf16 pair (s in the low half): o the
+ * largest bf16 up to the smallest value, s = (largest - o) / 15 rounded to fp32, then bf16, c = (x - o) / s rounded to the nearest
+ * (halves to even) and kept in 0 .. 15, all 0 where s is. A vector with an infinity or NaN, or a value below bf16's range, is NaN.
+ * write: row m's keys k[m ldk + head hk + i] and values into place[m] (outside the pool: the row is left out; the places of a call differ).
+ * read: what stands there, in bf16 or fp32 (outside: zeros). */
+size_t llj_kv4_block_bytes(int page, int dim, int vdim);
+int llj_kv4_write(const void* k, size_t ldk, size_t hk, const void* v, size_t ldv, size_t hv, const int* place, int M, int kv_heads, int dim,
+                  int vdim, int dt, void* pool, int pages, int page, void* stream);
+int llj_kv4_read(const void* pool, int pages, int page, const int* place, int M, int kv_heads, int dim, int vdim, int dt, void* k, size_t ldk,
+                 size_t hk, void* v, size_t ldv, size_t hv, void* stream);
+/* Grouped-query attention over it: rows q[m ldq + head dim + i], y of stride ldy, gates (NULL: none) of stride ldg. Row m sees the positions up
+ * to pos[m] (< 0: none, y = 0; page numbers outside the pool: none of that page) of its sequence's slot; scores q . k * scale, with sink one
+ * added to the denominator; y = sum p v * sigmoid(gate). work: `items` (first row, rows, sequence) of at most `rows` rows each (rows not in any
+ * item are left as they are); NULL: row m is sequence m, rows = 1. nsplit <= 64 key ranges; scratch part [M][heads][nsplit]
+ * [llj_kv4_part_width(vdim)] fp32 and count [items][llj_kv4_tiles] ints, zero before the first call (a call leaves them zero), for calls of
+ * one stream. */
+int llj_kv4_part_width(int vdim);
+int llj_kv4_tiles(int heads, int kv_heads, int rows);
+int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int* work, int items, int rows, const int* pos, const int* slot, int B,
+                   const int* table, int slots, int ldt, const void* pool, int pages, int page, float* part, int* count, int nsplit, void* y,
+                   int ldy, int M, int heads, int kv_heads, int dim, int vdim, float scale, int sink, int dt, void* stream);
+
 /* Measurement aid (no reference counterpart): reads `bytes` (a multiple of 16) at p once with
  * non-temporal 16-byte loads over `grid` workgroups of 256 and writes one float per workgroup to
  * out (grid floats). bench.py times it over a buffer far larger than the 256 MB MALL to report the

@@ -153,6 +153,14 @@ SIGNATURES = {
     "llj_gqa_decode": [_P, _I, _I, _I, _I, _I, _P, _I, _I, _F, _P, _P, _P, _I, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I,
                        _I, _I, _I, _I, _F, _I, _P],
     "llj_g_i8_linear": [_P, _I, _I, _I, _P, _P, _F, _P, _I, _P, _I, _P, _I, _I, _P],
+    "llj_pages_extend": [_P, _P, _I, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P],
+    "llj_pages_release": [_P, _I, _P, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P],
+    "llj_kv4_write": [_P, _U64, _U64, _P, _U64, _U64, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
+    "llj_kv4_read": [_P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _U64, _U64, _P, _U64, _U64, _P],
+    "llj_kv4_part_width": [_I],
+    "llj_kv4_tiles": [_I, _I, _I],
+    "llj_kv4_attend": [_P, _I, _P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I,
+                       _I, _P],
 }
 
 # workspace sizes (host functions)
@@ -167,6 +175,7 @@ SIZE_SIGNATURES = {
     "llj_g_linear_ws_bytes": [_I, _I, _I, _I, _I],
     "llj_gemm_ws_bytes": [_I, _I, _I, _I],
     "llj_gemm_bf16_ws_bytes": [_I, _I, _I],
+    "llj_kv4_block_bytes": [_I, _I, _I],
 }
 
 _lib = None
@@ -225,6 +234,15 @@ def call(name: str, *args) -> None:
     if rc != 0:
         what = "unsupported shape/argument (EINVAL)" if rc == 1000 else f"hipError {rc}"
         raise HipError(f"{name} failed: {what}")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call() on t's device and the current stream there, whichever device is the current one."""
+    st = torch.cuda.current_stream(t.device).cuda_stream
+    if t.device.index == torch.cuda.current_device():
+        return call(name, *args, st)
+    with torch.cuda.device(t.device):
+        call(name, *args, st)
 
 
 def g_linear(wkind: int, x, M: int, K: int, W, scales, zeros, bits: int, group: int, N: int, y, resid, dt: int, st: int) -> None:

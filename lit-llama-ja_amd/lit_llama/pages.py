@@ -1,0 +1,99 @@
+"""Block tables and slot maps of paged caches, made on the GPU from the requests' lengths (csrc/pages.hip).
+
+A page holds PAGE_SIZES tokens of one sequence. A sequence has a slot: `table[slot]` its pages in order, `seen[slot]` its tokens.
+`extend` gives the sequences of a call their new tokens: pages off the stack of free ones, and for every row of the call its
+sequence, position and place in the cache (page number * page + token in the page); nothing of it comes back to the host, so a captured
+step extends its sequences itself. `release` puts the pages of ended sequences back. A call that cannot be served (too few
+free pages, a slot twice, ...) has no rows -- all -1, which the cache's kernels leave out -- and changes no table: `PageRows.status`.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _hip
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+MAX_SEQUENCES = 4096  # of one call
+MAX_SLOTS = 65536
+NO_PAGES, BAD_CALL = 1, 2  # status bits
+
+
+@dataclass
+class PageRows:
+    """The rows of a call (int32, on the device). M may be more than the sequences' tokens: the rest are -1. `work`: items (first row, rows,
+    sequence) of at most `chunk` rows, those behind the last zero."""
+
+    row0: torch.Tensor  # (B + 1) first row of each sequence
+    item0: torch.Tensor  # (B + 1) first work item of each
+    row_seq: torch.Tensor  # (M)
+    pos: torch.Tensor  # (M)
+    place: torch.Tensor  # (M)
+    work: Optional[torch.Tensor]  # (M // chunk + B, 3)
+    seen: torch.Tensor  # (B) the sequences' tokens with those of this call
+    left: torch.Tensor  # (1) free pages behind it
+    status: torch.Tensor  # (1) 0, or NO_PAGES / BAD_CALL: the call was left undone
+
+
+def _ints(t: torch.Tensor, what: str, dims: int, device=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or not t.numel():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {dims} dimension(s) with elements")
+    if device is None:
+        _hip.require_device(t, what)
+    elif t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the tables on {device}")
+    return t
+
+
+def _tables(table, seen, free, nfree, slot, page) -> torch.device:
+    dev = _ints(table, "table", 2).device
+    for t, what in ((seen, "seen"), (free, "free"), (nfree, "nfree"), (slot, "slot")):
+        _ints(t, what, 1, dev)
+    if page not in PAGE_SIZES:
+        raise ValueError(f"pages of {page} tokens: {PAGE_SIZES} are taken")
+    if seen.numel() != table.shape[0] or nfree.numel() != 1:
+        raise ValueError(f"{seen.numel()} lengths and {nfree.numel()} counts for a table of {table.shape[0]} slots")
+    if table.shape[0] > MAX_SLOTS or slot.numel() > MAX_SEQUENCES or max(table.shape[1], free.numel()) * page > 1 << 30:
+        raise ValueError(f"up to {MAX_SLOTS} slots, {MAX_SEQUENCES} sequences a call and 2^30 tokens are taken, not {table.shape[0]}, "
+                         f"{slot.numel()} and {max(table.shape[1], free.numel()) * page}")
+    return dev
+
+
+def extend(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, slot: torch.Tensor, add: Optional[torch.Tensor],
+           M: int, page: int, chunk: int = 0, commit: bool = True, fault: Optional[torch.Tensor] = None) -> PageRows:
+    """add[b] more tokens (None: one) for the sequence in slot[b]. M: rows there is room for. commit False: lengths and stack stay as
+    they are (PageRows.seen and .left hold the new ones), and a later call makes the same rows again."""
+    dev = _tables(table, seen, free, nfree, slot, page)
+    B, M, chunk = slot.numel(), int(M), int(chunk)
+    if add is not None and _ints(add, "add", 1, dev).numel() != B:
+        raise ValueError(f"{add.numel()} counts for {B} sequences")
+    if fault is not None and _ints(fault, "fault", 1, dev).numel() != 1:
+        raise ValueError("fault is one int32")
+    if not 0 <= M <= 1 << 28 or chunk < 0:
+        raise ValueError(f"{M} rows in items of {chunk}")
+    n = M // chunk + B if chunk else 0
+    if n > 1 << 28:
+        raise ValueError(f"{n} work items")
+    o = torch.empty(3 * M + 3 * n + 3 * B + 4, dtype=torch.int32, device=dev)
+    parts = o.split([M, M, M, 3 * n, B + 1, B + 1, B, 1, 1])
+    row_seq, pos, place, work, row0, item0, after, left, status = parts
+    at = o.data_ptr()
+    rows, items, tail = at, at + 12 * M, at + 12 * (M + n)
+    _hip.call_on(table, "llj_pages_extend", slot.data_ptr(), _hip.ptr(add), B, seen.data_ptr(), table.shape[0], table.data_ptr(), table.shape[1],
+                 free.data_ptr(), nfree.data_ptr(), free.numel(), page, int(commit), tail, tail + 4 * (B + 1), rows, rows + 4 * M, rows + 8 * M, M,
+                 items, n, chunk, tail + 8 * (B + 1), tail + 8 * (B + 1) + 4 * B, tail + 8 * (B + 1) + 4 * B + 4, _hip.ptr(fault))
+    return PageRows(row0, item0, row_seq, pos, place, work.view(n, 3) if chunk else None, after, left, status)
+
+
+def release(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, slot: torch.Tensor, page: int,
+            fault: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The pages of these slots' sequences back onto the stack; the slots are empty behind it. Returns the status (1)."""
+    dev = _tables(table, seen, free, nfree, slot, page)
+    if fault is not None and _ints(fault, "fault", 1, dev).numel() != 1:
+        raise ValueError("fault is one int32")
+    status = torch.empty(1, dtype=torch.int32, device=dev)
+    _hip.call_on(table, "llj_pages_release", slot.data_ptr(), slot.numel(), seen.data_ptr(), table.shape[0], table.data_ptr(), table.shape[1],
+                 free.data_ptr(), nfree.data_ptr(), free.numel(), page, status.data_ptr(), _hip.ptr(fault))
+    return status

@@ -1,0 +1,429 @@
+"""The paged 4-bit K / V cache (csrc/kv4.hip, kv4_attend.hip) against oracle/kv4_np.py in double precision.
+
+Codes, scales and offsets are compared bit for bit. Attention's tolerance, for rows y = sum_j p_j v_j (derived, not fitted):
+  * the output's rounding, eps / 2 of its type, relative to |y|; the gate's sigmoid some fp32 roundings, 2^-21;
+  * a score is a sum of D products of bf16 numbers with 16 + c <= 31, accumulated in fp32, scaled, plus offset times the queries' sum:
+    |error| <= e = (D + 8) 2^-24 scale (31 s + |o|) sum |q| at most, the queries themselves exact (three bf16 terms);
+    every weight is then off by a factor exp(2 e) at most (its own score and the sum's), and by 2^-21 from exp2, whose argument is rounded: 2^-23
+    |score - top|, both times max |v|;
+  * a weight times its scale enters in two bf16 terms (2^-16) or three (2^-24) and is summed over n keys in fp32, n 2^-24, beside 16 + c: times
+    (31 s + |o|) of the values.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4_np as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32).cuda()
+
+
+def rounded(a, dtype):
+    """Values of the type, as numpy float64 and on the device."""
+    t = torch.tensor(np.asarray(a), dtype=torch.float32).to(dtype)
+    return t.double().numpy(), t.cuda()
+
+
+def keys(g, *shape):
+    """Channels of different spread around means of their own, a few of them large."""
+    mean = g.standard_normal(shape[1:]) * (1 + 6 * (g.random(shape[1:]) < 0.04))
+    return g.standard_normal(shape) * g.uniform(0.5, 1.5, shape[1:]) + mean
+
+
+def same(a, b):
+    return np.array_equal(a, b, equal_nan=True)
+
+
+# ------------------------------------------------------------------------------------------- rows in and out
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,G,D,V,page", [(1, 1, 64, 64, 16), (5, 2, 128, 128, 64), (33, 3, 78, 78, 16), (70, 2, 1, 3, 32), (19, 1, 256, 200, 128),
+                                          (300, 4, 96, 64, 256), (9, 2, 65, 129, 64), (40, 10, 64, 64, 16), (7, 1, 128, 250, 16), (1003, 5, 24, 8, 32)])
+def test_rows_in_and_out(hip, dtype, M, G, D, V, page):
+    """The bytes of every page, and what is read back in both types; the pages between are left as they were."""
+    from lit_llama import kv4
+
+    g = np.random.default_rng(M + D)
+    lay = kv4.Layout(G, D, V, page)
+    n = -(-M // page) + 2
+    pool = lay.pool(n)
+    pool.fill_(0xA5)
+    k, kd = rounded(keys(g, M, G, D), dtype)
+    v, vd = rounded(g.standard_normal((M, G, V)), dtype)
+    place = g.permutation(n * page)[:M]
+    kv4.write(pool, lay, kd, vd, ints(place))
+    want = np.full((n, G, lay.block_bytes()), 0xA5, np.uint8)
+    kb, vb = O.width(D) // 2, O.width(V) // 2
+    for m, at in enumerate(place):
+        p, t = divmod(int(at), page)
+        for h in range(G):
+            b = O.pack(k[m, h][None], v[m, h][None], page)
+            c, s = page * kb, page * (kb + vb)
+            for base, size in ((0, kb), (c, vb), (s, 4), (s + 4 * page, 4)):
+                want[p, h, base + t * size:base + (t + 1) * size] = b[base:base + size]
+    assert np.array_equal(pool.cpu().numpy(), want)
+    for out in DTYPES:
+        a, b = kv4.read(pool, lay, ints(place), out)
+        assert same(a.double().cpu().numpy(), rounded(O.stands_for(k), out)[0])
+        assert same(b.double().cpu().numpy(), rounded(O.stands_for(v), out)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_vectors_on_the_edges(hip, dtype):
+    """Constant vectors, values on the border between two codes, zeros of both signs, subnormal spreads, the type's largest values, a large
+    common part, infinities and NaN in one vector beside good ones."""
+    from lit_llama import kv4
+
+    D, G = 64, 1
+    top = float(torch.finfo(dtype).max)
+    g = np.random.default_rng(3)
+    x = np.zeros((14, G, D))
+    x[1] = 1.375
+    x[2] = -0.0
+    x[3, 0] = np.linspace(-7.5, 7.5, D)  # (o = -7.5, s = 1: every half is a border)
+    x[3, 0, ::4] = 0.0
+    x[4, 0] = np.arange(D) % 31 * 0.5
+    x[5, 0, ::2], x[5, 0, 1] = top, -3.3e38
+    x[6, 0, 3] = 1e-39
+    x[7, 0] = 1000 + g.standard_normal(D)
+    x[8, 0, 5] = np.inf
+    x[9, 0, 5] = -np.inf
+    x[10, 0, 5] = np.nan
+    x[11, 0] = g.standard_normal(D) * 1e-30
+    x[12, 0] = -top
+    x[13, 0] = np.where(np.arange(D) % 2, 1e-30, -1.0)
+    k, kd = rounded(x, dtype)
+    lay = kv4.Layout(G, D, D, 16)
+    pool = lay.pool(1)
+    kv4.write(pool, lay, kd, kd, ints(np.arange(14)))
+    a, b = kv4.read(pool, lay, ints(np.arange(14)))
+    with np.errstate(over="ignore"):  # (code 15 of the widest vector stands for more than a float32 holds)
+        want = O.stands_for(k).astype(np.float32).astype(np.float64)
+    assert same(a.double().cpu().numpy(), want) and same(b.double().cpu().numpy(), want)
+    assert np.isnan(want[8:11]).all() and np.isfinite(O.stands_for(k)[:8]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_places_outside(hip, dtype):
+    """Rows out of packed projections at odd columns, heads with gaps, rows whose place is -1 or behind the pool."""
+    from lit_llama import kv4
+
+    g = np.random.default_rng(5)
+    M, G, D, V = 21, 3, 40, 24
+    lay = kv4.Layout(G, D, V, 16)
+    wide, wd = rounded(keys(g, M, G * (D + V) + 7), dtype)
+    k, v = wd[:, 3:3 + G * D], wd[:, 3 + G * D:3 + G * (D + V)]
+    place = np.arange(M) + 5
+    place[4], place[9], place[15] = -1, 48, 1 << 30
+    pool = lay.pool(3)
+    pool.fill_(0x5A)
+    kv4.write(pool, lay, k, v, ints(place))
+    a, b = kv4.read(pool, lay, ints(place))
+    good = np.array([0 <= p < 48 for p in place])
+    wk = O.stands_for(wide[:, 3:3 + G * D].reshape(M, G, D))
+    wv = O.stands_for(wide[:, 3 + G * D:3 + G * (D + V)].reshape(M, G, V))
+    assert same(a.double().cpu().numpy()[good], wk[good].astype(np.float32)) and same(b.double().cpu().numpy()[good], wv[good].astype(np.float32))
+    assert not a[torch.tensor(~good).cuda()].any() and not b[torch.tensor(~good).cuda()].any()
+    used = set(place[good])
+    left, _ = kv4.read(pool, lay, ints([p for p in range(48) if p not in used]))
+    assert torch.equal(left, left[:1, :1].expand_as(left))  # (the filling, everywhere else)
+    # heads with gaps between them
+    gaps, gd = rounded(keys(g, M, G, D + V + 1), dtype)
+    kv4.write(pool, lay, gd[:, :, 1:1 + D], gd[:, :, 1 + D:], ints(np.arange(M)))
+    a, b = kv4.read(pool, lay, ints(np.arange(M)))
+    assert same(a.double().cpu().numpy(), O.stands_for(gaps[:, :, 1:1 + D]).astype(np.float32))
+    assert same(b.double().cpu().numpy(), O.stands_for(gaps[:, :, 1 + D:]).astype(np.float32))
+
+
+# ------------------------------------------------------------------------------------------- attention
+class Case:
+    """Sequences of `lens` tokens in scattered pages; the last rows[b] of each are the rows of the call (0: none)."""
+
+    def __init__(self, lens, rows, H, G, D, V, page, dtype, seed=0, spread=1.0):
+        from lit_llama import kv4
+
+        g = self.g = np.random.default_rng(seed)
+        self.lens, self.rows, self.H, self.dtype, self.page = lens, rows, H, dtype, page
+        self.lay = lay = kv4.Layout(G, D, V, page)
+        need = [-(-n // page) for n in lens]
+        pages = sum(need) + 3
+        order = list(g.permutation(pages))
+        B = len(lens)
+        table = np.full((B + 2, max(need + [1]) + 1), -1)
+        slots = g.permutation(B + 2)[:B]
+        self.pool = lay.pool(pages)
+        # places nobody wrote hold NaN pairs
+        page_bytes = page * (O.width(D) + O.width(V)) // 2
+        self.pool[:, :, page_bytes:] = 0xFF
+        self.k, self.v = [], []
+        for b, n in enumerate(lens):
+            ids = [order.pop() for _ in range(need[b])]
+            table[slots[b], :need[b]] = ids
+            k, kd = rounded(keys(g, n, G, D), torch.bfloat16)
+            v, vd = rounded(g.standard_normal((n, G, V)), torch.bfloat16)
+            if n:
+                kv4.write(self.pool, lay, kd, vd, ints([ids[t // page] * page + t % page for t in range(n)]))
+            self.k.append(O.stands_for(k))
+            self.v.append(O.stands_for(v))
+        self.table, self.slot = ints(table), ints(slots)
+        self.M = sum(rows)
+        self.pos = [n - r + i for n, r in zip(lens, rows) for i in range(r)]
+        self.seq = [b for b, r in enumerate(rows) for _ in range(r)]
+        self.q, self.qd = rounded(spread * g.standard_normal((self.M, H * D)), dtype)
+        self.gate, self.gated = rounded(g.standard_normal((self.M, H)), dtype)
+
+    def work(self, per):
+        out, first = [], 0
+        for b, r in enumerate(self.rows):
+            out += [[first + j, min(per, r - j), b] for j in range(0, r, per)]
+            first += r
+        return ints(out)
+
+    def want(self, scale=None, sink=False, gate=False):
+        D, V, H = self.lay.dim, self.lay.vdim, self.H
+        scale = D ** -0.5 if scale is None else scale
+        y, tol = np.zeros((self.M, H, V)), np.zeros((self.M, H, 1))
+        half = float(torch.finfo(self.dtype).eps) / 2
+        terms = 2.0 ** -16 if self.dtype == torch.bfloat16 else 2.0 ** -24
+        R = H // self.lay.kv_heads
+        for m in range(self.M):
+            b, p = self.seq[m], self.pos[m]
+            q = self.q[m].reshape(1, H, D)
+            y[m] = O.attend(q, self.k[b], self.v[b], [p], scale, sink, self.gate[m][None] if gate else None)[0]
+            if p < 0:
+                continue
+            for h in range(H):
+                k, v = self.k[b][:p + 1, h // R], self.v[b][:p + 1, h // R]
+                ks, vs = np.abs(k).max() + 31 * (k.max() - k.min()) / 15, np.abs(v).max() + 31 * (v.max() - v.min()) / 15
+                e = (D + 8) * 2.0 ** -24 * scale * ks * np.abs(q[0, h]).sum()
+                s = k @ q[0, h] * scale
+                spread = max(s.max(), 0.0) - min(s.min(), 0.0)
+                tol[m, h] = np.abs(v).max() * (np.expm1(2 * e) + 2.0 ** -21 + 2.0 ** -22 * spread) + vs * (terms + (p + 1) * 2.0 ** -24)
+        return y.reshape(self.M, -1), (tol + (half + 2.0 ** -21) * np.abs(y)).reshape(self.M, -1)
+
+    def run(self, per=None, q=None, **kw):
+        from lit_llama import kv4
+
+        if kw.pop("gate", False):
+            kw["gate"] = self.gated
+        if per is not None:
+            kw.update(work=self.work(per), rows=per)
+        return kv4.attend(self.qd if q is None else q, self.pool, self.lay, self.table, self.slot, ints(self.pos), **kw)
+
+    def check(self, y, **kw):
+        want, tol = self.want(**kw)
+        off = np.abs(y.double().cpu().numpy().reshape(want.shape) - want)
+        assert (off <= tol).all(), f"{(off > tol).sum()} of {off.size} outside, the worst {np.max(off / np.maximum(tol, 1e-300)):.3g} of its bound"
+
+
+SIZES = [(4, 2, 64, 64, 16), (8, 2, 128, 128, 64), (2, 2, 128, 128, 128), (6, 3, 78, 78, 32), (20, 1, 96, 64, 16), (5, 1, 40, 200, 64), (3, 3, 256, 256, 16),
+         (34, 2, 130, 66, 256), (2, 1, 1, 1, 16), (4, 4, 33, 17, 128), (4, 2, 200, 90, 32), (2, 2, 64, 160, 16), (2, 1, 160, 48, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D,V,page", SIZES)
+def test_steps(hip, dtype, H, G, D, V, page):
+    """One row per sequence: a first token, ends inside a tile and a page, exactly on them, one behind; an idle place."""
+    c = Case([1, 2, 15, 16, 17, 63, 64, 65, 0, 128, 257, 300], [1] * 12, H, G, D, V, page, dtype, seed=D + V)
+    c.check(c.run())
+    c.check(c.run(scale=0.05, sink=True, gate=True), scale=0.05, sink=True, gate=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D,V,page", SIZES)
+@pytest.mark.parametrize("per", [1, 3, 40, 200])
+def test_rows_of_several_tokens(hip, dtype, H, G, D, V, page, per):
+    """Prompt rows and portions behind earlier tokens in items of every size; a sequence without rows between."""
+    c = Case([5, 40, 1, 33, 150], [5, 7, 1, 0, 70], H, G, D, V, page, dtype, seed=H)
+    c.check(c.run(per))
+    c.check(c.run(per, sink=True, gate=True), sink=True, gate=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1023, 4096, 20001])
+def test_long_sequences(hip, dtype, n):
+    """Key ranges over several workgroups, and queries with a few keys that win."""
+    c = Case([n, 700], [1, 1], 8, 2, 128, 128, 64, dtype, seed=n, spread=3.0)
+    c.check(c.run())
+    c = Case([n, 700], [3, 2], 4, 2, 64, 64, 16, dtype, seed=n)
+    c.check(c.run(4, sink=True), sink=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_prompt(hip, dtype):
+    c = Case([900, 130], [333, 130], 4, 2, 128, 128, 64, dtype, seed=8)
+    c.check(c.run(64, gate=True), gate=True)
+    c = Case([700], [700], 3, 1, 64, 64, 32, dtype, seed=9)
+    c.check(c.run(42, sink=True), sink=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_see_nothing(hip, dtype):
+    """pos < 0 (also below -1), slots outside the tables and pages outside the pool: zero rows, with and without ranges and a sink; a gap in
+    the middle of a table hides its own tokens only."""
+    c = Case([600, 600, 40], [1, 1, 1], 4, 2, 64, 64, 16, dtype)
+    from lit_llama import kv4
+
+    pos = ints([-1, 599, -7])
+    for sink in (False, True):
+        y = kv4.attend(c.qd, c.pool, c.lay, c.table, c.slot, pos, sink=sink)
+        assert not y[0].any() and not y[2].any() and y[1].any()
+    bad = ints([c.slot[0].item(), -1, 5])
+    y = kv4.attend(c.qd, c.pool, c.lay, c.table, bad, ints(c.pos))
+    assert y[0].any() and not y[1].any() and not y[2].any()
+    t = c.table.clone()
+    t[c.slot[0].item()] = 1 << 20
+    t[c.slot[1].item(), 7] = -1
+    y = kv4.attend(c.qd, c.pool, c.lay, t, c.slot, ints(c.pos))
+    assert not y[0].any()
+    keep = [j for j in range(600) if not 7 * 16 <= j < 8 * 16]
+    c.k[1], c.v[1] = c.k[1][keep], c.v[1][keep]
+    c.pos[1] = len(keep) - 1
+    want, tol = c.want()
+    assert (np.abs(y.double().cpu().numpy() - want) <= tol)[1:].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("per", [None, 8])
+def test_what_stands_behind_a_row_is_not_read(hip, dtype, per):
+    """NaN keys and values at later positions of the same page do not reach a row, in rows of one call either; NaN at a visible one does."""
+    from lit_llama import kv4
+
+    c = Case([30], [1] if per is None else [6], 2, 1, 64, 64, 32, dtype)
+    at = int(c.table[c.slot[0].item(), 0]) * 32
+    nan = torch.full((1, 1, 64), float("nan"), dtype=dtype, device="cuda")
+    if per is None:
+        kv4.write(c.pool, c.lay, nan, nan, ints([at + 30]))
+        c.check(c.run())
+        kv4.write(c.pool, c.lay, nan, nan, ints([at + 11]))
+        assert c.run().isnan().all()
+    else:
+        kv4.write(c.pool, c.lay, nan, nan, ints([at + 27]))  # the rows are positions 24 .. 29
+        y = c.run(per)
+        assert y[3:].isnan().all()
+        want, tol = c.want()
+        assert (np.abs(y.double().cpu().numpy() - want) <= tol)[:3].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_rows_and_outputs(hip, dtype):
+    """Queries and gates out of packed projections at odd columns, into a wider output; rows of no item are left as they were."""
+    c = Case([100, 41, 7], [1, 1, 1], 6, 2, 64, 64, 16, dtype, seed=2)
+    wide = torch.zeros(3, 6 * 64 + 6 + 5, dtype=dtype, device="cuda")
+    wide[:, 3:3 + 384] = c.qd
+    wide[:, 387:393] = c.gated
+    out = torch.full((3, 400), 7.0, dtype=dtype, device="cuda")
+    from lit_llama import kv4
+
+    kv4.attend(wide[:, 3:387], c.pool, c.lay, c.table, c.slot, ints(c.pos), gate=wide[:, 387:393], out=out[:, 5:389])
+    c.check(out[:, 5:389], gate=True)
+    assert (out[:, :5] == 7).all() and (out[:, 389:] == 7).all()
+    out.fill_(7.0)
+    kv4.attend(c.qd, c.pool, c.lay, c.table, c.slot, ints(c.pos), out=out[:, :384], work=ints([[2, 1, 2], [0, 0, 0], [0, 1, 0]]), rows=1)
+    want, tol = c.want()
+    assert (np.abs(out[:, :384].double().cpu().numpy() - want) <= tol)[[0, 2]].all() and (out[1] == 7).all()
+    # items that name no rows of the call
+    out.fill_(7.0)
+    kv4.attend(c.qd, c.pool, c.lay, c.table, c.slot, ints(c.pos), out=out[:, :384], work=ints([[3, 1, 0], [-1, 1, 0], [0, 1, 3], [2, 2, 0], [0, -4, 0]]), rows=2)
+    assert (out == 7).all()
+
+
+def test_kept_counters_and_graphs(hip):
+    """Counters that a program keeps, over calls of different sizes; a captured call replayed over new rows and lengths, with eager
+    calls between."""
+    from lit_llama import kv4
+
+    c = Case([3000, 2500], [1, 1], 8, 2, 128, 128, 64, torch.bfloat16, seed=4)
+    count = torch.zeros(64, dtype=torch.int32, device="cuda")
+    q, pos = c.qd.clone(), ints(c.pos)
+    kv4.attend(q, c.pool, c.lay, c.table, c.slot, pos, count=count)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = kv4.attend(q, c.pool, c.lay, c.table, c.slot, pos, count=count)
+    g = np.random.default_rng(0)
+    for turn in range(4):
+        c.pos = [int(g.integers(0, 3000)), int(g.integers(-1, 2500))]
+        c.q, qd = rounded(g.standard_normal(c.q.shape), torch.bfloat16)
+        q.copy_(qd)
+        pos.copy_(ints(c.pos))
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(y)
+        e = kv4.attend(qd, c.pool, c.lay, c.table, c.slot, ints(c.pos), count=count)
+        assert torch.equal(e, y) and not count.any()
+        small = Case([700], [1], 2, 2, 64, 64, 16, torch.float32, seed=turn)
+        small.check(small.run(count=count))
+        assert not count.any()
+
+
+def test_two_streams(hip):
+    """Calls on two streams at once, each with counters of its own."""
+    a = Case([5000, 4000], [1, 1], 8, 2, 128, 128, 64, torch.bfloat16, seed=5)
+    b = Case([2500], [1], 4, 4, 64, 64, 16, torch.float32, seed=6)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ya, yb = [], []
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            ya.append(a.run())
+        with torch.cuda.stream(s2):
+            yb.append(b.run())
+    torch.cuda.synchronize()
+    a.check(ya[0])
+    b.check(yb[0])
+    assert all(torch.equal(y, ya[0]) for y in ya) and all(torch.equal(y, yb[0]) for y in yb)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 64])
+def test_a_serving_run(hip, dtype, page):
+    """The operators together: unequal prompts, steps, a portion, one request ending and another taking its slot and pages."""
+    from lit_llama import kv4, pages
+
+    g = np.random.default_rng(page)
+    H, G, D, V = 8, 2, 64, 64
+    lay = kv4.Layout(G, D, V, page)
+    n_pages = 400 // page + 6
+    table, seen = ints(np.full((4, 300 // page + 1), -1)), ints([0] * 4)
+    free, nfree, fault = ints(g.permutation(n_pages)), ints([n_pages]), ints([0])
+    pool = lay.pool(n_pages)
+    keep = {s: ([], []) for s in range(4)}
+
+    def call(slots, adds):
+        M = sum(adds)
+        r = pages.extend(table, seen, free, nfree, ints(slots), ints(adds), M, page, chunk=8, fault=fault)
+        q, qd = rounded(g.standard_normal((M, H * D)), dtype)
+        k, kd = rounded(keys(g, M, G, D), dtype)
+        v, vd = rounded(g.standard_normal((M, G, V)), dtype)
+        kv4.write(pool, lay, kd, vd, r.place)
+        step = max(adds) == 1
+        y = kv4.attend(qd, pool, lay, table, ints(slots), r.pos, work=None if step else r.work, rows=1 if step else 8)
+        c = Case.__new__(Case)
+        c.lay, c.H, c.dtype, c.M, c.q, c.seq, c.pos, c.k, c.v = lay, H, dtype, M, q, [], [], [], []
+        row = 0
+        for b, (s, n) in enumerate(zip(slots, adds)):
+            keep[s][0].extend(O.stands_for(k[row:row + n]))
+            keep[s][1].extend(O.stands_for(v[row:row + n]))
+            c.k.append(np.array(keep[s][0]))
+            c.v.append(np.array(keep[s][1]))
+            c.pos += range(len(keep[s][0]) - n, len(keep[s][0]))
+            c.seq += [b] * n
+            row += n
+        assert r.pos.tolist() == c.pos
+        c.check(y)
+
+    call([2, 0, 3], [37, 1, 90])
+    for _ in range(3):
+        call([0, 3, 2], [1, 1, 1])
+    call([3, 0], [20, 65])
+    assert int(pages.release(table, seen, free, nfree, ints([3]), page, fault)) == 0
+    keep[3] = ([], [])
+    call([1, 3], [64, 33])
+    for _ in range(2):
+        call([3, 1, 0, 2], [1, 1, 1, 1])
+    assert int(fault) == 0
