@@ -679,10 +679,11 @@ int llj_kv4_read(const void* pool, int pages, int page, const int* place, int M,
  * to pos[m] (< 0: none, y = 0; page numbers outside the pool: none of that page) of its sequence's slot; scores q . k * scale, with sink one
  * added to the denominator; y = sum p v * sigmoid(gate). work: `items` (first row, rows, sequence) of at most `rows` rows each (rows not in any
  * item are left as they are); NULL: row m is sequence m, rows = 1. nsplit <= 64 key ranges; scratch part [M][heads][nsplit]
- * [llj_kv4_part_width(vdim)] fp32 and count [items][llj_kv4_tiles] ints, zero before the first call (a call leaves them zero), for calls of
+ * [llj_kv4_part_width(vdim)] fp32 and count [items][llj_kv4_tiles] (0: sizes
+ * not taken; the workgroups of an item and range) ints, zero before the first call (a call leaves them zero), for calls of
  * one stream. */
 int llj_kv4_part_width(int vdim);
-int llj_kv4_tiles(int heads, int kv_heads, int rows);
+int llj_kv4_tiles(int heads, int kv_heads, int dim, int vdim, int rows, int dt);
 int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int* work, int items, int rows, const int* pos, const int* slot, int B,
                    const int* table, int slots, int ldt, const void* pool, int pages, int page, float* part, int* count, int nsplit, void* y,
                    int ldy, int M, int heads, int kv_heads, int dim, int vdim, float scale, int sink, int dt, void* stream);

@@ -1,0 +1,373 @@
+// Attention of prompt rows over the paged 4-bit cache (mathematics: kv4_attend.h).
+//
+// One workgroup per (item, K / V head, key range): the item's columns, (row, query head) pairs, 16 QB to a wave, so a tile of keys and values is
+// taken out of its codes once for up to 64 QB columns. Tiles of 64 keys: each wave fetches and unpacks 16 of them, into the order in which
+// the product's operands are read (16 bytes a lane, no bank conflicts on reading), two buffers, so that the next tile's codes are in flight over
+// this one's products and one barrier a tile is enough. Scores, softmax and weights stay in registers: S^T = K q^T leaves a
+// column's weights where O^T = V^T P^T wants them. Workgroups of one head are 8 apart and so on one XCD, whose L2 holds its pages; items
+// are taken from the last, which see the most keys.
+#include <type_traits>
+
+#include "kv4_attend.h"
+#include "lit_llama_amd.h"
+
+namespace llj {
+
+template <int KT, int VH>
+struct Kv4Tile {
+  static constexpr int kKeys = 4 * KT * 1024, kValues = 8 * VH * 1024;  // bytes of unpacked keys, values
+  static constexpr int kPairs = kKeys + kValues, kTop = kPairs + 1024, kBytes = kTop + 16;  // (pairs: key scales, offsets, value scales, offsets)
+};
+
+template <typename T, int KT, int VH, int QB>
+__global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_kernel(Kv4Attend p) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 2 : 1;
+  constexpr int KB = 16 * KT, VB = 32 * VH, VW = 64 * VH, VD = VH >= 2 ? VH / 2 : 1;
+  typedef Kv4Tile<KT, VH> Tile;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two tiles; 64 floats a column at the end
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
+  constexpr int CW = 64 * QB;  // columns
+  const int R = p.H / p.pool.G, CB = (p.rows * R + CW - 1) / CW, x = p.items * CB - 1 - blockIdx.x / p.pool.G;
+  const int gh = blockIdx.x % p.pool.G, item = x / CB, cb = x % CB, sp = blockIdx.y;
+  int r0 = item, n = 1, b = item;
+  if (p.work) {
+    r0 = p.work[3 * (size_t)item];
+    n = p.work[3 * (size_t)item + 1];
+    b = p.work[3 * (size_t)item + 2];
+  }
+  n = n < p.rows ? n : p.rows;
+  if (n <= 0 || r0 < 0 || r0 > p.M - n || b < 0 || b >= p.B) return;  // (uniform; no such rows)
+  const Kv4Columns cols{r0, gh, R, cb * CW, n * R - cb * CW < CW ? n * R - cb * CW : CW};
+  if (cols.n <= 0) return;
+  const int sl = p.slot[b];
+  const bool held = sl >= 0 && sl < p.slots;
+  const kv4_row tab = scalar_row(p.table + (size_t)(held ? uniform(sl) : 0) * p.ldt);
+  const int k = p.pool.k, pmask = (1 << k) - 1, most = held ? (p.ldt << k) - 1 : -1;
+  // the last position any column sees (a lane a column)
+  int plast = -1;
+  for (int i = lane; i < cols.n; i += 64) {
+    const int o = p.pos[r0 + (cols.c0 + i) / R];
+    plast = o > plast ? o : plast;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_xor(plast, d, 64);
+    plast = o > plast ? o : plast;
+  }
+  plast = uniform(plast < most ? plast : most);
+  const int tiles = plast < 0 ? 0 : plast / 64 + 1, per = (tiles + p.nsplit - 1) / p.nsplit;
+  const int t0 = sp * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+  // ---- this wave's columns
+  int row[QB], head[QB], pc[QB], wlast = -1, wfirst = 0x7fffffff;
+  u32x4 qf[QB][NQ][KT];
+  float qs[QB], qi[QB];
+  const float sl2 = kv4_scale(p), slack = kSlack / sl2;
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const int c = (wave * QB + q) * 16 + col;
+    cols.at(c < cols.n ? c : cols.n - 1, row[q], head[q]);
+    pc[q] = p.pos[row[q]];
+    pc[q] = pc[q] < most ? pc[q] : most;
+    wlast = pc[q] > wlast ? pc[q] : wlast;
+    wfirst = pc[q] < wfirst ? pc[q] : wfirst;
+    qs[q] = kv4_query<T, KT, NQ>(p, row[q], head[q], g, qf[q]);
+    qi[q] = F32 ? 0.f : -16.f * qs[q];
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    const int o = __shfl_xor(wlast, d, 64), f = __shfl_xor(wfirst, d, 64);
+    wlast = o > wlast ? o : wlast;
+    wfirst = f < wfirst ? f : wfirst;
+  }
+  wlast = wave * QB * 16 < cols.n ? uniform(wlast) : -1;  // (a wave without columns only unpacks)
+  wfirst = uniform(wfirst);
+
+  // ---- a tile's codes: this wave's 16 keys of it
+  uint32_t kw[KT], vw[4][VD], pair;
+  bool ok;
+  auto page_of = [&](int t) {
+    const int at = (64 * t + 16 * wave) >> k;
+    return tab[at < p.ldt ? at : p.ldt - 1];
+  };
+  auto fetch = [&](int t, int id) {
+    ok = id >= 0 && id < p.pool.pages;
+    const int off = (64 * t + 16 * wave) & pmask;
+    const uint8_t* blk = p.pool.p + ((size_t)(ok ? id : 0) * p.pool.G + gh) * p.pool.blk;
+    const uint8_t* ka = blk + (off + col) * KB + 4 * KT * g;
+    if constexpr (KT == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(ka);
+      kw[0] = x.x;
+      kw[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < KT / 4; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(ka + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kw[4 * i + e] = x[e];
+      }
+    }
+    const uint8_t* va = blk + p.pool.vc + (off + 4 * g) * VB + 2 * VH * col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VH == 1) {
+        vw[i][0] = *reinterpret_cast<const uint16_t*>(va + i * VB);
+      } else if constexpr (VH == 2) {
+        vw[i][0] = *reinterpret_cast<const uint32_t*>(va + i * VB);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(va + i * VB);
+        vw[i][0] = x.x;
+        vw[i][1] = x.y;
+      }
+    }
+    pair = *reinterpret_cast<const uint32_t*>(blk + (lane & 16 ? p.pool.vs : p.pool.ks) + 4 * (off + col));
+    if (!ok || 64 * t + 16 * wave + col > plast) pair = 0;  // (behind the last row's position stands anything)
+  };
+  auto unpack = [&](uint8_t* buf) {
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) *reinterpret_cast<u32x4*>(buf + (kk * 4 + wave) * 1024 + lane * 16) = codes_bf<F32>(kw[kk]);
+    uint8_t* vb = buf + Tile::kKeys + (wave >> 1) * 4 * VH * 1024 + lane * 16 + 8 * (wave & 1);
+#pragma unroll
+    for (int v = 0; v < VH; ++v) {
+      uint32_t x[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if constexpr (VH == 1) x[e] = vw[2 * e][0] | vw[2 * e + 1][0] << 16;
+        else x[e] = __builtin_amdgcn_perm(vw[2 * e + 1][v / 2], vw[2 * e][v / 2], v % 2 ? 0x07060302u : 0x05040100u);
+      }
+      const u32x4 a = codes_h<true>(x[0]), c = codes_h<true>(x[1]);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) *reinterpret_cast<uint2*>(vb + (4 * v + d) * 1024) = make_uint2(a[d], c[d]);
+    }
+    const float sc = bflo(pair), of = bfhi(pair) + (F32 || lane >= 16 ? 8.f * sc : 0.f);  // (codes c - 8)
+    if (lane < 32) {
+      float* at = reinterpret_cast<float*>(buf + Tile::kPairs + (lane >> 4) * 512) + wave * 16 + col;
+      at[0] = sc;
+      at[64] = of;
+    }
+    const float top = row16_max(sc);  // of the values' scales in lanes 16 .. 31; -1: keys that are not there
+    if (lane == 16) *reinterpret_cast<float*>(buf + Tile::kTop + 4 * wave) = ok ? top : -1.f;
+  };
+
+  float m_run[QB], l_run[QB], z_run[QB], unit = kScaleMin, up = weight_unit(unit);
+  f32x4 acc[QB][4 * VH];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    m_run[q] = -INFINITY;
+    l_run[q] = z_run[q] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 4 * VH; ++d) acc[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int next = 0;
+  if (t0 < t1) {
+    fetch(t0, page_of(t0));
+    next = page_of(t0 + 1);
+    unpack(lds);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const uint8_t* buf = lds + ((t - t0) & 1) * Tile::kBytes;
+    if (t + 1 < t1) {
+      fetch(t + 1, next);
+      next = page_of(t + 2);
+    }
+    if (64 * t <= wlast) {  // (uniform in the wave)
+      f32x4 s[QB][4];
+#pragma unroll
+      for (int q = 0; q < QB; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[q][j] = f32x4{qi[q], qi[q], qi[q], qi[q]};
+      // Operands are read two steps of the sum (8 of them) ahead of their products; the fences keep the compiler from reading each right before its
+      // use, which left the LDS latency open 30 times a tile (4,096 rows of 32 heads: 222 us with that)
+      u32x4 a[2][8];
+      f32x4 sc[4], of[4];
+      const f32x4* pairs = reinterpret_cast<const f32x4*>(buf + Tile::kPairs) + g;
+      auto keys = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[c & 1][i] = *reinterpret_cast<const u32x4*>(buf + (8 * c + i) * 1024 + lane * 16);
+      };
+      keys(0);
+#pragma unroll
+      for (int c = 0; c < KT / 2; ++c) {
+        if (c + 1 < KT / 2) keys(c + 1);
+        else
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[j] = pairs[4 * j];
+            of[j] = pairs[16 + 4 * j];
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int q = 0; q < QB; ++q)
+#pragma unroll
+            for (int e = 0; e < NQ; ++e)
+              s[q][i & 3] = mfma_bf16(__builtin_bit_cast(bf16x8, a[c & 1][i]), __builtin_bit_cast(bf16x8, qf[q][e][2 * c + (i >> 2)]), s[q][i & 3]);
+      }
+      const f32x4 tops = *reinterpret_cast<const f32x4*>(buf + Tile::kTop);
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      const bool gap = uniform(fminf(fminf(tops[0], tops[1]), fminf(tops[2], tops[3])) < 0.f);
+      const bool masked = gap || 64 * t + 63 > wfirst;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < QB; ++q) s[q][j] = kv4_scores(s[q][j], sc[j], of[j], qs[q]);
+      if (masked) {
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int lim = tops[j] < 0.f ? -1 : pc[q];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (64 * t + 16 * j + 4 * g + i > lim) s[q][j][i] = -INFINITY;
+          }
+      }
+      float mx[QB];
+      bool raise = top > unit + unit;
+#pragma unroll
+      for (int q = 0; q < QB; ++q) {
+        mx[q] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[q] = fmaxf(mx[q], s[q][j][i]);
+        mx[q] = groups_max(mx[q]);
+        raise |= mx[q] > m_run[q] + slack;
+      }
+      if (__any(raise)) {  // a new maximum, or larger scales
+        const float grown = fmaxf(unit, pow2_floor(top));
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+          const float m_new = fmaxf(m_run[q], mx[q]);
+          float corr = m_run[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[q] - m_new) * sl2);
+          m_run[q] = m_new;
+          l_run[q] *= corr;
+          z_run[q] *= corr;
+          corr *= unit / grown;
+#pragma unroll
+          for (int d = 0; d < 4 * VH; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[q][d][i] *= corr;
+        }
+        unit = grown;
+        up = weight_unit(unit);
+      }
+      u32x4 va[2][4 * VH];
+      f32x4 sv[4], zv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sv[j] = pairs[32 + 4 * j];
+        zv[j] = pairs[48 + 4 * j];
+      }
+      auto values = [&](int u) {
+#pragma unroll
+        for (int d = 0; d < 4 * VH; ++d) va[u][d] = *reinterpret_cast<const u32x4*>(buf + Tile::kKeys + (u * 4 * VH + d) * 1024 + lane * 16);
+      };
+      uint32_t pt[QB][4][2][NP];
+      auto weights = [&](auto some) {  // (some: keys that a column does not see, whose values may be NaN)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 su = sv[j] * up;
+#pragma unroll
+          for (int q = 0; q < QB; ++q) {
+            const float mu = m_run[q] == -INFINITY ? 0.f : m_run[q], mus = mu * sl2;
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float e = kv4_weight<F32>(s[q][j][i], mu, mus, sl2);
+              const bool seen = !some || s[q][j][i] != -INFINITY;
+              l_run[q] += e;
+              z_run[q] = fmaf(e, seen ? zv[j][i] : 0.f, z_run[q]);
+              w[i] = e * (seen ? su[i] : 0.f);
+            }
+            split_h<NP>(w[0], w[1], pt[q][j][0]);
+            split_h<NP>(w[2], w[3], pt[q][j][1]);
+          }
+        }
+      };
+      if (masked) weights(std::true_type{});
+      else weights(std::false_type{});
+      values(0);  // (the scores' registers are free now)
+      values(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < 4 * VH; ++d)
+#pragma unroll
+          for (int q = 0; q < QB; ++q)
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+              acc[q][d] = mfma_f16(va[u][d], u32x4{pt[q][2 * u][0][i], pt[q][2 * u][1][i], pt[q][2 * u + 1][0][i], pt[q][2 * u + 1][1][i]}, acc[q][d]);
+    }
+    if (t + 1 < t1) unpack(lds + ((t + 1 - t0) & 1) * Tile::kBytes);  // (its last readers passed the barrier before this tile)
+    __syncthreads();
+  }
+  // ---- lane (col, g) holds values VW / 4 g + 4 VH i + 4 v + d of its columns
+  const float down = unit * kUnweight;
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const float l = groups_sum(l_run[q]), z = groups_sum(z_run[q]), m = m_run[q] * sl2;
+    if ((wave * QB + q) * 16 + col < cols.n) {
+      const float f = p.nsplit == 1 ? kv4_factor<T>(p, row[q], head[q], m, l) : 1.f;
+      float* dst = p.nsplit == 1 ? nullptr : kv4_part<VW>(p, row[q], head[q], sp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < VH; ++v) {
+          const int at = VW / 4 * g + 4 * VH * i + 4 * v;
+          f32x4 o;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] = fmaf(acc[q][4 * v + d][i], down, z);
+          if (p.nsplit == 1) {
+            kv4_store<T>(p, row[q], head[q], at, o * f);
+          } else {
+            put2(dst + at, o[0], o[1]);
+            put2(dst + at + 2, o[2], o[3]);
+          }
+        }
+      if (p.nsplit > 1 && g == 0) put2(dst + VW, m, l);
+    }
+  }
+  if (p.nsplit > 1) kv4_merge<T, VW>(p, cols, p.count + (size_t)x * p.pool.G + gh, reinterpret_cast<float*>(lds));
+}
+
+// 16-column blocks a wave: two where their accumulators and queries leave room for two workgroups on a CU
+constexpr int kv4_blocks(int D, int V, int dt) { return dt == 0 && D <= 128 && V <= 128 ? 2 : 1; }
+int kv4_flash_tiles(int columns, int D, int V, int dt) { return (columns + 64 * kv4_blocks(D, V, dt) - 1) / (64 * kv4_blocks(D, V, dt)); }
+
+template <typename T, int KT, int VH>
+static int kv4_flash_go(const Kv4Attend& p, hipStream_t s) {
+  constexpr int QB = kv4_blocks(32 * KT, 64 * VH, sizeof(T) == 4);
+  auto kern = kv4_flash_kernel<T, KT, VH, QB>;
+  constexpr size_t tiles = 2 * Kv4Tile<KT, VH>::kBytes, join = (size_t)64 * QB * 64 * 4, lds = tiles > join ? tiles : join;
+  if constexpr (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  const int CB = (p.rows * (p.H / p.pool.G) + 64 * QB - 1) / (64 * QB);
+  hipLaunchKernelGGL(kern, dim3((unsigned)p.items * CB * p.pool.G, p.nsplit), dim3(256), lds, s, p);
+  LLJ_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int KT>
+static int kv4_flash_values(const Kv4Attend& p, hipStream_t s) {
+  if (p.V <= 64) return kv4_flash_go<T, KT, 1>(p, s);
+  if (p.V <= 128) return kv4_flash_go<T, KT, 2>(p, s);
+  return kv4_flash_go<T, KT, 4>(p, s);
+}
+
+template <typename T>
+static int kv4_flash_keys(const Kv4Attend& p, hipStream_t s) {
+  if (p.D <= 64) return kv4_flash_values<T, 2>(p, s);
+  if (p.D <= 128) return kv4_flash_values<T, 4>(p, s);
+  return kv4_flash_values<T, 8>(p, s);
+}
+
+int kv4_flash(const Kv4Attend& p, int dt, hipStream_t s) { return dt == 0 ? kv4_flash_keys<bf16_t>(p, s) : kv4_flash_keys<float>(p, s); }
+
+}  // namespace llj

@@ -37,63 +37,76 @@ class PageRows:
     status: torch.Tensor  # (1) 0, or NO_PAGES / BAD_CALL: the call was left undone
 
 
-def _ints(t: torch.Tensor, what: str, dims: int, device=None) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or not t.numel():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of {dims} dimension(s) with elements")
-    if device is None:
+def on_device(t: torch.Tensor, what: str) -> int:
+    """The index of t's GPU."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what} is no tensor")
+    index = t.get_device()
+    if index < 0:
         _hip.require_device(t, what)
-    elif t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the tables on {device}")
-    return t
+    return index
 
 
-def _tables(table, seen, free, nfree, slot, page) -> torch.device:
-    dev = _ints(table, "table", 2).device
-    for t, what in ((seen, "seen"), (free, "free"), (nfree, "nfree"), (slot, "slot")):
-        _ints(t, what, 1, dev)
+def ints(t: torch.Tensor, what: str, dims: int, index: int) -> int:
+    """Checks a contiguous int32 tensor with elements on device `index`; how many it has. (Few calls into torch: a decode step's
+    wrappers take as long as its small kernels.)"""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or not (n := t.numel()):
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {dims} dimension(s) with elements")
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, other operands on cuda:{index}")
+    return n
+
+
+def _tables(table, seen, free, nfree, slot, page) -> tuple:
+    """(device, slots, pages a slot, sequences, pages)"""
+    index = table.get_device() if isinstance(table, torch.Tensor) else -1
+    ints(table, "table", 2, index)
+    on_device(table, "table")
+    slots, width = table.shape
+    B, cap = ints(slot, "slot", 1, index), ints(free, "free", 1, index)
     if page not in PAGE_SIZES:
         raise ValueError(f"pages of {page} tokens: {PAGE_SIZES} are taken")
-    if seen.numel() != table.shape[0] or nfree.numel() != 1:
-        raise ValueError(f"{seen.numel()} lengths and {nfree.numel()} counts for a table of {table.shape[0]} slots")
-    if table.shape[0] > MAX_SLOTS or slot.numel() > MAX_SEQUENCES or max(table.shape[1], free.numel()) * page > 1 << 30:
-        raise ValueError(f"up to {MAX_SLOTS} slots, {MAX_SEQUENCES} sequences a call and 2^30 tokens are taken, not {table.shape[0]}, "
-                         f"{slot.numel()} and {max(table.shape[1], free.numel()) * page}")
-    return dev
+    if ints(seen, "seen", 1, index) != slots or ints(nfree, "nfree", 1, index) != 1:
+        raise ValueError(f"{seen.numel()} lengths and {nfree.numel()} counts for a table of {slots} slots")
+    if slots > MAX_SLOTS or B > MAX_SEQUENCES or max(width, cap) * page > 1 << 30:
+        raise ValueError(f"up to {MAX_SLOTS} slots, {MAX_SEQUENCES} sequences a call and 2^30 tokens are taken, not {slots}, {B} and "
+                         f"{max(width, cap) * page}")
+    return index, slots, width, B, cap
 
 
 def extend(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, slot: torch.Tensor, add: Optional[torch.Tensor],
            M: int, page: int, chunk: int = 0, commit: bool = True, fault: Optional[torch.Tensor] = None) -> PageRows:
     """add[b] more tokens (None: one) for the sequence in slot[b]. M: rows there is room for. commit False: lengths and stack stay as
     they are (PageRows.seen and .left hold the new ones), and a later call makes the same rows again."""
-    dev = _tables(table, seen, free, nfree, slot, page)
-    B, M, chunk = slot.numel(), int(M), int(chunk)
-    if add is not None and _ints(add, "add", 1, dev).numel() != B:
+    index, slots, width, B, cap = _tables(table, seen, free, nfree, slot, page)
+    if add is not None and ints(add, "add", 1, index) != B:
         raise ValueError(f"{add.numel()} counts for {B} sequences")
-    if fault is not None and _ints(fault, "fault", 1, dev).numel() != 1:
+    if fault is not None and ints(fault, "fault", 1, index) != 1:
         raise ValueError("fault is one int32")
     if not 0 <= M <= 1 << 28 or chunk < 0:
         raise ValueError(f"{M} rows in items of {chunk}")
     n = M // chunk + B if chunk else 0
     if n > 1 << 28:
         raise ValueError(f"{n} work items")
-    o = torch.empty(3 * M + 3 * n + 3 * B + 4, dtype=torch.int32, device=dev)
-    parts = o.split([M, M, M, 3 * n, B + 1, B + 1, B, 1, 1])
-    row_seq, pos, place, work, row0, item0, after, left, status = parts
-    at = o.data_ptr()
-    rows, items, tail = at, at + 12 * M, at + 12 * (M + n)
-    _hip.call_on(table, "llj_pages_extend", slot.data_ptr(), _hip.ptr(add), B, seen.data_ptr(), table.shape[0], table.data_ptr(), table.shape[1],
-                 free.data_ptr(), nfree.data_ptr(), free.numel(), page, int(commit), tail, tail + 4 * (B + 1), rows, rows + 4 * M, rows + 8 * M, M,
-                 items, n, chunk, tail + 8 * (B + 1), tail + 8 * (B + 1) + 4 * B, tail + 8 * (B + 1) + 4 * B + 4, _hip.ptr(fault))
+    o = torch.empty(3 * M + 3 * n + 3 * B + 4, dtype=torch.int32, device=table.device)
+    row_seq, pos, place, work, row0, item0, after, left, status = o.split_with_sizes([M, M, M, 3 * n, B + 1, B + 1, B, 1, 1])
+    rows = o.data_ptr()
+    items = rows + 12 * M
+    tail = items + 12 * n
+    ends = tail + 8 * (B + 1)
+    _hip.call_on(index, "llj_pages_extend", slot.data_ptr(), None if add is None else add.data_ptr(), B, seen.data_ptr(), slots, table.data_ptr(), width,
+                 free.data_ptr(), nfree.data_ptr(), cap, page, int(commit), tail, tail + 4 * (B + 1), rows, rows + 4 * M, rows + 8 * M, M,
+                 items, n, chunk, ends, ends + 4 * B, ends + 4 * B + 4, None if fault is None else fault.data_ptr())
     return PageRows(row0, item0, row_seq, pos, place, work.view(n, 3) if chunk else None, after, left, status)
 
 
 def release(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, slot: torch.Tensor, page: int,
             fault: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The pages of these slots' sequences back onto the stack; the slots are empty behind it. Returns the status (1)."""
-    dev = _tables(table, seen, free, nfree, slot, page)
-    if fault is not None and _ints(fault, "fault", 1, dev).numel() != 1:
+    index, slots, width, B, cap = _tables(table, seen, free, nfree, slot, page)
+    if fault is not None and ints(fault, "fault", 1, index) != 1:
         raise ValueError("fault is one int32")
-    status = torch.empty(1, dtype=torch.int32, device=dev)
-    _hip.call_on(table, "llj_pages_release", slot.data_ptr(), slot.numel(), seen.data_ptr(), table.shape[0], table.data_ptr(), table.shape[1],
-                 free.data_ptr(), nfree.data_ptr(), free.numel(), page, status.data_ptr(), _hip.ptr(fault))
+    status = torch.empty(1, dtype=torch.int32, device=table.device)
+    _hip.call_on(index, "llj_pages_release", slot.data_ptr(), B, seen.data_ptr(), slots, table.data_ptr(), width, free.data_ptr(), nfree.data_ptr(),
+                 cap, page, status.data_ptr(), _hip.ptr(fault))
     return status

@@ -67,8 +67,12 @@ def test_tiles_and_ranges():
     from lit_llama import kv4
 
     L = lib()
-    assert L.llj_kv4_tiles(8, 2, 1) == 2 and L.llj_kv4_tiles(8, 2, 5) == 4 and L.llj_kv4_tiles(34, 2, 1) == 4
-    assert L.llj_kv4_tiles(8, 3, 1) == 0 and L.llj_kv4_tiles(0, 1, 1) == 0 and L.llj_kv4_tiles(8, 2, 0) == 0 and L.llj_kv4_tiles(65535, 1, 65535) == 0
+    def tiles(heads, kv_heads, rows, dim=64, vdim=64, dt=0):
+        return L.llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt)
+
+    assert tiles(8, 2, 1) == 2 and tiles(8, 2, 5) == 4 and tiles(34, 2, 1) == 4
+    assert tiles(8, 2, 32) == 2 and tiles(8, 2, 33) == 4 and tiles(8, 2, 32, dt=1) == 4 and tiles(8, 2, 32, vdim=200) == 4
+    assert tiles(8, 3, 1) == 0 and tiles(0, 1, 1) == 0 and tiles(8, 2, 0) == 0 and tiles(65535, 1, 65535) == 0 and tiles(8, 2, 1, dim=300) == 0
     lay = kv4.Layout(8, 128, 128, 64)
     for items, keys in ((1, 10), (1, 300), (1, 1 << 20), (8, 4096), (64, 8192), (4096, 1 << 20)):
         n, need = kv4.splits(lay, 32, items, 1, keys)
@@ -111,7 +115,7 @@ def test_attention_refuses():
            dict(table=None), dict(slots=0), dict(ldt=0), dict(ldt=1 << 27), dict(pool=None), dict(pool=P + 4), dict(pages=0), dict(page=30), dict(part=None),
            dict(count=None), dict(part=P + 4), dict(nsplit=0), dict(nsplit=65), dict(y=None), dict(ldy=255), dict(M=-1), dict(heads=0), dict(heads=3),
            dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(vdim=0), dict(vdim=260), dict(dt=2), dict(work=None), dict(work=None, rows=1, items=5, M=5),
-           dict(work=None, rows=1, items=3, M=2, B=4), dict(heads=40000, kv_heads=20000, ldq=1 << 30)]
+           dict(work=None, rows=1, items=3, M=2, B=4), dict(heads=70000, kv_heads=35000, ldq=1 << 30)]
     for b in bad:
         assert lib().llj_kv4_attend(*{**good, **b}.values()) == EINVAL, b
     assert lib().llj_kv4_attend(*{**good, "items": 0}.values()) == 0
