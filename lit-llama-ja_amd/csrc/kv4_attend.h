@@ -165,15 +165,15 @@ __device__ __forceinline__ float* kv4_part(const Kv4Attend& p, int row, int head
 // The last of the ranges' workgroups merges them, in range order: device-scope stores, a wait for them, one device-scope counter per tile,
 // device-scope loads; nobody waits for another workgroup, and the last one resets the counter. lds: 64 floats a column.
 template <typename T, int VW>
-__device__ void kv4_merge(const Kv4Attend& p, const Kv4Columns& cs, int* counter, float* lds) {
+__device__ void kv4_merge(const Kv4Attend& p, const Kv4Columns& cs, int ranges, int* counter, float* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   __shared__ int last;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
     const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = done == p.nsplit - 1;
-    if (done == p.nsplit - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = done == ranges - 1;
+    if (done == ranges - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!last) return;
@@ -182,7 +182,7 @@ __device__ void kv4_merge(const Kv4Attend& p, const Kv4Columns& cs, int* counter
     cs.at(c, row, head);
     const float* pr = kv4_part<VW>(p, row, head, 0);
     float2 st = make_float2(-INFINITY, 0.f);
-    if (lane < p.nsplit) st = get2(pr + (size_t)lane * (VW + 4) + VW);
+    if (lane < ranges) st = get2(pr + (size_t)lane * (VW + 4) + VW);
     const float m = wave_max(st.x), mu = m == -INFINITY ? 0.f : m;
     const float w = __builtin_amdgcn_exp2f(st.x - mu);
     lds[c * 64 + lane] = w * kv4_factor<T>(p, row, head, m, wave_sum(w * st.y));
@@ -194,17 +194,17 @@ __device__ void kv4_merge(const Kv4Attend& p, const Kv4Columns& cs, int* counter
     cs.at(c, row, head);
     const float* pr = kv4_part<VW>(p, row, head, 0) + v;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.nsplit; s += 8) {
+    for (int s = 0; s < ranges; s += 8) {
       float2 a[8], b[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float* q = pr + (size_t)(s + e < p.nsplit ? s + e : p.nsplit - 1) * (VW + 4);
+        const float* q = pr + (size_t)(s + e < ranges ? s + e : ranges - 1) * (VW + 4);
         a[e] = get2(q);
         b[e] = get2(q + 2);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (s + e < p.nsplit) o += f32x4{a[e].x, a[e].y, b[e].x, b[e].y} * lds[c * 64 + s + e];
+        if (s + e < ranges) o += f32x4{a[e].x, a[e].y, b[e].x, b[e].y} * lds[c * 64 + s + e];
     }
     kv4_store<T>(p, row, head, v, o);
   }

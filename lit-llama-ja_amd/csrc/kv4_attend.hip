@@ -54,7 +54,10 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   }
   plast = uniform(plast);
   pfirst = uniform(pfirst);
-  const int steps = plast < 0 ? 0 : plast / STEP + 1, per = (steps + p.nsplit - 1) / p.nsplit;
+  // as many ranges as there are rounds of the four waves: what the caller sized for the longest sequence costs a short one nothing
+  const int steps = plast < 0 ? 0 : plast / STEP + 1, rounds = (steps + 3) / 4, ranges = rounds < 1 ? 1 : rounds < p.nsplit ? rounds : p.nsplit;
+  if (sp >= ranges) return;
+  const int per = (steps + ranges - 1) / ranges;
   const int s0 = sp * per, s1 = s0 + per < steps ? s0 + per : steps;
 
   u32x4 qf[NQ][KT];
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     }
     int rr, hh;
     cols.at(cc, rr, hh);
-    if (p.nsplit == 1) {
+    if (ranges == 1) {
       kv4_store<T>(p, rr, hh, v, o * kv4_factor<T>(p, rr, hh, mx, l));
     } else {
       float* dst = kv4_part<VW>(p, rr, hh, sp);
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
       if (v == 0) put2(dst + VW, mx, l);
     }
   }
-  if (p.nsplit > 1) kv4_merge<T, VW>(p, cols, p.count + (size_t)item * gridDim.y + blockIdx.y, red);
+  if (ranges > 1) kv4_merge<T, VW>(p, cols, ranges, p.count + (size_t)item * gridDim.y + blockIdx.y, red);
 }
 
 template <typename T, int KT, int VH>
@@ -358,7 +361,7 @@ int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int*
   LLJ_REQUIRE(kv4_sizes(pool, pages, page, kv_heads, dim, vdim, dt) && q && pos && slot && table && y && items >= 0 && rows >= 1 && rows <= 65535 &&
               B >= 1 && slots >= 1 && ldt >= 1 && ldt <= (1 << 30) / page && M >= 0 && heads >= 1 && heads % kv_heads == 0 && heads <= 65535 &&
               ldq >= heads * dim && ldy >= heads * vdim && (!gate || ldg >= heads) && nsplit >= 1 && nsplit <= 64 && (nsplit == 1 || (part && count)) &&
-              (((uintptr_t)part | (uintptr_t)count) & 7) == 0 && (work || (rows == 1 && items <= M && items <= B)));
+              ((uintptr_t)part & 15) == 0 && ((uintptr_t)count & 3) == 0 && (work || (rows == 1 && items <= M && items <= B)));
   const int tiles = llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt);
   LLJ_REQUIRE(tiles > 0 && (long long)items * tiles <= 0x7fffffff);
   if (items == 0 || M == 0) return 0;

@@ -16,7 +16,7 @@ namespace llj {
 template <int KT, int VH>
 struct Kv4Tile {
   static constexpr int kKeys = 4 * KT * 1024, kValues = 8 * VH * 1024;  // bytes of unpacked keys, values
-  static constexpr int kPairs = kKeys + kValues, kTop = kPairs + 1024, kBytes = kTop + 16;  // (pairs: key scales, offsets, value scales, offsets)
+  static constexpr int kPairs = kKeys + kValues, kTop = kPairs + 1024, kBytes = kTop + 32;  // (pairs: key scales, offsets, value scales, offsets)
 };
 
 template <typename T, int KT, int VH, int QB>
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 2 : 1;
   constexpr int KB = 16 * KT, VB = 32 * VH, VW = 64 * VH, VD = VH >= 2 ? VH / 2 : 1;
   typedef Kv4Tile<KT, VH> Tile;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two tiles; 64 floats a column at the end
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two tiles
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
   constexpr int CW = 64 * QB;  // columns
   const int R = p.H / p.pool.G, CB = (p.rows * R + CW - 1) / CW, x = p.items * CB - 1 - blockIdx.x / p.pool.G;
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   if (cols.n <= 0) return;
   const int sl = p.slot[b];
   const bool held = sl >= 0 && sl < p.slots;
-  const kv4_row tab = scalar_row(p.table + (size_t)(held ? uniform(sl) : 0) * p.ldt);
+  const int* tab = p.table + (size_t)(held ? sl : 0) * p.ldt + vzero();  // (loaded into vector registers, moved to scalar ones a tile later: a move at the load would wait for it)
   const int k = p.pool.k, pmask = (1 << k) - 1, most = held ? (p.ldt << k) - 1 : -1;
   // the last position any column sees (a lane a column)
   int plast = -1;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   const int t0 = sp * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
   // ---- this wave's columns
-  int row[QB], head[QB], pc[QB], wlast = -1, wfirst = 0x7fffffff;
+  int row[QB], head[QB], pc[QB], wfirst = 0x7fffffff;
   u32x4 qf[QB][NQ][KT];
   float qs[QB], qi[QB];
   const float sl2 = kv4_scale(p), slack = kSlack / sl2;
@@ -70,23 +70,20 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
     cols.at(c < cols.n ? c : cols.n - 1, row[q], head[q]);
     pc[q] = p.pos[row[q]];
     pc[q] = pc[q] < most ? pc[q] : most;
-    wlast = pc[q] > wlast ? pc[q] : wlast;
     wfirst = pc[q] < wfirst ? pc[q] : wfirst;
     qs[q] = kv4_query<T, KT, NQ>(p, row[q], head[q], g, qf[q]);
     qi[q] = F32 ? 0.f : -16.f * qs[q];
   }
 #pragma unroll
   for (int d = 1; d < 16; d <<= 1) {
-    const int o = __shfl_xor(wlast, d, 64), f = __shfl_xor(wfirst, d, 64);
-    wlast = o > wlast ? o : wlast;
+    const int f = __shfl_xor(wfirst, d, 64);
     wfirst = f < wfirst ? f : wfirst;
   }
-  wlast = wave * QB * 16 < cols.n ? uniform(wlast) : -1;  // (a wave without columns only unpacks)
   wfirst = uniform(wfirst);
 
   // ---- a tile's codes: this wave's 16 keys of it
   uint32_t kw[KT], vw[4][VD], pair;
-  bool ok;
+  bool ok = false;
   auto page_of = [&](int t) {
     const int at = (64 * t + 16 * wave) >> k;
     return tab[at < p.ldt ? at : p.ldt - 1];
@@ -140,14 +137,12 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
       for (int d = 0; d < 4; ++d) *reinterpret_cast<uint2*>(vb + (4 * v + d) * 1024) = make_uint2(a[d], c[d]);
     }
-    const float sc = bflo(pair), of = bfhi(pair) + (F32 || lane >= 16 ? 8.f * sc : 0.f);  // (codes c - 8)
-    if (lane < 32) {
-      float* at = reinterpret_cast<float*>(buf + Tile::kPairs + (lane >> 4) * 512) + wave * 16 + col;
-      at[0] = sc;
-      at[64] = of;
-    }
-    const float top = row16_max(sc);  // of the values' scales in lanes 16 .. 31; -1: keys that are not there
-    if (lane == 16) *reinterpret_cast<float*>(buf + Tile::kTop + 4 * wave) = ok ? top : -1.f;
+    const float sc = bflo(pair), of = bfhi(pair) + (F32 || lane & 16 ? 8.f * sc : 0.f);  // (codes c - 8)
+    float* at = reinterpret_cast<float*>(buf + Tile::kPairs + (lane & 16) * 32) + wave * 16 + col;  // (lanes 32 .. 63 write the same)
+    at[0] = sc;
+    at[64] = of;
+    const float top = row16_max(sc);  // of the values' scales in the odd rows of lanes; -1: keys that are not there. (The keys' go behind)
+    *reinterpret_cast<float*>(buf + Tile::kTop + 16 - (lane & 16) + 4 * wave) = ok ? top : -1.f;
   };
 
   float m_run[QB], l_run[QB], z_run[QB], unit = kScaleMin, up = weight_unit(unit);
@@ -159,27 +154,28 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
     for (int d = 0; d < 4 * VH; ++d) acc[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // Tile t is multiplied while tile t + 1 goes from registers to LDS, between the first products, and tile t + 2 is on its way to registers
   int next = 0;
+  auto last = [&](int t) { return t < t1 ? t : t1 - 1; };
   if (t0 < t1) {
-    fetch(t0, page_of(t0));
-    next = page_of(t0 + 1);
+    fetch(t0, uniform(page_of(t0)));
+    next = page_of(last(t0 + 1));
     unpack(lds);
+    fetch(last(t0 + 1), uniform(next));
+    next = page_of(last(t0 + 2));
   }
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const uint8_t* buf = lds + ((t - t0) & 1) * Tile::kBytes;
-    if (t + 1 < t1) {
-      fetch(t + 1, next);
-      next = page_of(t + 2);
-    }
-    if (64 * t <= wlast) {  // (uniform in the wave)
+    uint8_t* then = lds + ((t + 1 - t0) & 1) * Tile::kBytes;  // (its last readers passed the barrier before this tile)
+    {
       f32x4 s[QB][4];
 #pragma unroll
       for (int q = 0; q < QB; ++q)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[q][j] = f32x4{qi[q], qi[q], qi[q], qi[q]};
-      // Operands are read two steps of the sum (8 of them) ahead of their products; the fences keep the compiler from reading each right before its
-      // use, which left the LDS latency open 30 times a tile (4,096 rows of 32 heads: 222 us with that)
+      // Operands are read ahead of their products, fences keep the compiler from reading each right before its use (which left the LDS latency
+      // open 30 times a tile)
       u32x4 a[2][8];
       f32x4 sc[4], of[4];
       const f32x4* pairs = reinterpret_cast<const f32x4*>(buf + Tile::kPairs) + g;
@@ -187,17 +183,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[c & 1][i] = *reinterpret_cast<const u32x4*>(buf + (8 * c + i) * 1024 + lane * 16);
       };
-      keys(0);
-#pragma unroll
-      for (int c = 0; c < KT / 2; ++c) {
-        if (c + 1 < KT / 2) keys(c + 1);
-        else
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            sc[j] = pairs[4 * j];
-            of[j] = pairs[16 + 4 * j];
-          }
-        __builtin_amdgcn_sched_barrier(0);
+      auto products = [&](int c) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -205,7 +191,23 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
             for (int e = 0; e < NQ; ++e)
               s[q][i & 3] = mfma_bf16(__builtin_bit_cast(bf16x8, a[c & 1][i]), __builtin_bit_cast(bf16x8, qf[q][e][2 * c + (i >> 2)]), s[q][i & 3]);
+      };
+      keys(0);
+#pragma unroll
+      for (int c = 0; c < KT / 2; ++c) {
+        if (c + 1 < KT / 2) keys(c + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c == 0) unpack(then);
+        products(c);
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[j] = pairs[4 * j];
+        of[j] = pairs[16 + 4 * j];
+      }
+      fetch(last(t + 2), uniform(next));
+      next = page_of(last(t + 3));
       const f32x4 tops = *reinterpret_cast<const f32x4*>(buf + Tile::kTop);
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       const bool gap = uniform(fminf(fminf(tops[0], tops[1]), fminf(tops[2], tops[3])) < 0.f);
@@ -259,51 +261,53 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
       f32x4 sv[4], zv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        sv[j] = pairs[32 + 4 * j];
+        sv[j] = pairs[32 + 4 * j] * up;
         zv[j] = pairs[48 + 4 * j];
       }
+      auto weights = [&](int q, auto some, uint32_t (&pt)[4][2][NP]) {  // (some: keys that a column does not see, whose values may be NaN)
+        const float mu = m_run[q] == -INFINITY ? 0.f : m_run[q], mus = mu * sl2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = kv4_weight<F32>(s[q][j][i], mu, mus, sl2);
+            const bool seen = !some || s[q][j][i] != -INFINITY;
+            l_run[q] += e;
+            z_run[q] = fmaf(e, seen ? zv[j][i] : 0.f, z_run[q]);
+            w[i] = e * (seen ? sv[j][i] : 0.f);
+          }
+          split_h<NP>(w[0], w[1], pt[j][0]);
+          split_h<NP>(w[2], w[3], pt[j][1]);
+        }
+      };
       auto values = [&](int u) {
 #pragma unroll
         for (int d = 0; d < 4 * VH; ++d) va[u][d] = *reinterpret_cast<const u32x4*>(buf + Tile::kKeys + (u * 4 * VH + d) * 1024 + lane * 16);
       };
-      uint32_t pt[QB][4][2][NP];
-      auto weights = [&](auto some) {  // (some: keys that a column does not see, whose values may be NaN)
+      auto add = [&](int q, int u, const uint32_t (&pt)[4][2][NP]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 su = sv[j] * up;
+        for (int d = 0; d < 4 * VH; ++d)
 #pragma unroll
-          for (int q = 0; q < QB; ++q) {
-            const float mu = m_run[q] == -INFINITY ? 0.f : m_run[q], mus = mu * sl2;
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float e = kv4_weight<F32>(s[q][j][i], mu, mus, sl2);
-              const bool seen = !some || s[q][j][i] != -INFINITY;
-              l_run[q] += e;
-              z_run[q] = fmaf(e, seen ? zv[j][i] : 0.f, z_run[q]);
-              w[i] = e * (seen ? su[i] : 0.f);
-            }
-            split_h<NP>(w[0], w[1], pt[q][j][0]);
-            split_h<NP>(w[2], w[3], pt[q][j][1]);
-          }
-        }
+          for (int i = 0; i < NP; ++i)
+            acc[q][d] = mfma_f16(va[u][d], u32x4{pt[2 * u][0][i], pt[2 * u][1][i], pt[2 * u + 1][0][i], pt[2 * u + 1][1][i]}, acc[q][d]);
       };
-      if (masked) weights(std::true_type{});
-      else weights(std::false_type{});
+      uint32_t pt[QB][4][2][NP];
+      if (masked) {
+#pragma unroll
+        for (int q = 0; q < QB; ++q) weights(q, std::true_type{}, pt[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < QB; ++q) weights(q, std::false_type{}, pt[q]);
+      }
       values(0);  // (the scores' registers are free now)
       values(1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int d = 0; d < 4 * VH; ++d)
-#pragma unroll
-          for (int q = 0; q < QB; ++q)
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-              acc[q][d] = mfma_f16(va[u][d], u32x4{pt[q][2 * u][0][i], pt[q][2 * u][1][i], pt[q][2 * u + 1][0][i], pt[q][2 * u + 1][1][i]}, acc[q][d]);
+        for (int q = 0; q < QB; ++q) add(q, u, pt[q]);
     }
-    if (t + 1 < t1) unpack(lds + ((t + 1 - t0) & 1) * Tile::kBytes);  // (its last readers passed the barrier before this tile)
     __syncthreads();
   }
   // ---- lane (col, g) holds values VW / 4 g + 4 VH i + 4 v + d of its columns
@@ -322,17 +326,50 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
           f32x4 o;
 #pragma unroll
           for (int d = 0; d < 4; ++d) o[d] = fmaf(acc[q][4 * v + d][i], down, z);
-          if (p.nsplit == 1) {
-            kv4_store<T>(p, row[q], head[q], at, o * f);
-          } else {
-            put2(dst + at, o[0], o[1]);
-            put2(dst + at + 2, o[2], o[3]);
-          }
+          if (p.nsplit == 1) kv4_store<T>(p, row[q], head[q], at, o * f);
+          else *reinterpret_cast<f32x4*>(dst + at) = o;
         }
-      if (p.nsplit > 1 && g == 0) put2(dst + VW, m, l);
+      if (p.nsplit > 1 && g == 0) {
+        dst[VW] = m;
+        dst[VW + 1] = l;
+      }
     }
   }
-  if (p.nsplit > 1) kv4_merge<T, VW>(p, cols, p.count + (size_t)x * p.pool.G + gh, reinterpret_cast<float*>(lds));
+}
+
+// The ranges of a prompt's columns put together by a launch of their own, a wave a column (partials of 128 columns by device-scope stores and a last
+// workgroup, as for few rows, took longer than the attention: 512 rows in two ranges 67 us, in one 28).
+template <typename T, int VW, int CW>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attend p) {
+  constexpr int N = VW / 64;  // values a lane
+  const int R = p.H / p.pool.G, CB = (p.rows * R + CW - 1) / CW, x = blockIdx.x / p.pool.G, gh = blockIdx.x % p.pool.G;
+  const int item = x / CB, lane = threadIdx.x & 63, c = x % CB * CW + blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  int r0 = item, n = 1, b = item;
+  if (p.work) {
+    r0 = p.work[3 * (size_t)item];
+    n = p.work[3 * (size_t)item + 1];
+    b = p.work[3 * (size_t)item + 2];
+  }
+  n = n < p.rows ? n : p.rows;
+  if (n <= 0 || r0 < 0 || r0 > p.M - n || b < 0 || b >= p.B || c >= n * R) return;
+  const int row = r0 + c / R, head = gh * R + c % R;
+  const float* pr = kv4_part<VW>(p, row, head, 0);
+  float m = -INFINITY, l = 0.f;
+  if (lane < p.nsplit) {  // nsplit <= 64
+    m = pr[(size_t)lane * (VW + 4) + VW];
+    l = pr[(size_t)lane * (VW + 4) + VW + 1];
+  }
+  const float top = wave_max(m), w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top)), f = w * kv4_factor<T>(p, row, head, top, wave_sum(w * l));
+  float o[N] = {};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float ws = __shfl(f, s, 64);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = fmaf(ws, pr[(size_t)s * (VW + 4) + N * lane + i], o[i]);
+  }
+  T* y = (T*)p.y + (size_t)row * p.ldy + (size_t)head * p.V;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (N * lane + i < p.V) stv(y, N * lane + i, o[i]);
 }
 
 // 16-column blocks a wave: two where their accumulators and queries leave room for two workgroups on a CU
@@ -343,13 +380,14 @@ template <typename T, int KT, int VH>
 static int kv4_flash_go(const Kv4Attend& p, hipStream_t s) {
   constexpr int QB = kv4_blocks(32 * KT, 64 * VH, sizeof(T) == 4);
   auto kern = kv4_flash_kernel<T, KT, VH, QB>;
-  constexpr size_t tiles = 2 * Kv4Tile<KT, VH>::kBytes, join = (size_t)64 * QB * 64 * 4, lds = tiles > join ? tiles : join;
+  constexpr size_t lds = 2 * Kv4Tile<KT, VH>::kBytes;
   if constexpr (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return (int)e;
   }
   const int CB = (p.rows * (p.H / p.pool.G) + 64 * QB - 1) / (64 * QB);
   hipLaunchKernelGGL(kern, dim3((unsigned)p.items * CB * p.pool.G, p.nsplit), dim3(256), lds, s, p);
+  if (p.nsplit > 1) hipLaunchKernelGGL((kv4_join_kernel<T, 64 * VH, 64 * QB>), dim3((unsigned)p.items * CB * p.pool.G, 16 * QB), dim3(256), 0, s, p);
   LLJ_CHECK_LAUNCH();
   return 0;
 }

@@ -50,33 +50,45 @@ __device__ __forceinline__ int find_seq(const int* at, int n, int x) {
   return lo;
 }
 
-// exclusive sums of three values over the workgroup; total in `sum`
-__device__ __forceinline__ void scan3(int (&v)[3], int (&sum)[3], int (*part)[3]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  int in[3] = {v[0], v[1], v[2]};
+// v plus the values that the lanes before hold (saturating), through the lanes' neighbours: 6 steps of one move and one sum
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+  return sat_add(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);         // the end of rows 0 and 2 to 1 and 3
+  return scan_step<0x143, 0xC>(v);      // of row 1 to 2 and 3
+}
+
+// exclusive sums of three values over the workgroup (right unless they saturate, and then nothing is taken); total in `sum`. part: zero
+// behind the workgroup's waves.
+__device__ __forceinline__ void scan3(int (&v)[3], int (&sum)[3], int4 (*part)) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int in[3];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
+  for (int i = 0; i < 3; ++i) in[i] = wave_scan(v[i]);
+  __syncthreads();  // the last call's readers of part are done
+  if (lane == 63) part[wave] = make_int4(in[0], in[1], in[2], 0);
+  __syncthreads();
+  int before[3] = {0, 0, 0}, all[3] = {0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    const int4 x = part[w];
+    const int a[3] = {x.x, x.y, x.z};
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const int o = __shfl_up(in[i], d, 64);
-      if (lane >= d) in[i] = sat_add(in[i], o);
+      before[i] = w == wave ? all[i] : before[i];
+      all[i] = sat_add(all[i], a[i]);
     }
   }
-  __syncthreads();  // the last call's readers of part are done
-  if (lane == 63)
-    for (int i = 0; i < 3; ++i) part[wave][i] = in[i];
-  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    int before = 0, all = 0;
-    for (int w = 0; w < nw; ++w) {
-      if (w == wave) before = all;
-      all = sat_add(all, part[w][i]);
-    }
-    // (not in - v: where the sums saturate, nothing is taken)
-    const int up = __shfl_up(in[i], 1, 64);
-    v[i] = sat_add(before, lane ? up : 0);
-    sum[i] = all;
+    v[i] = sat_add(before[i], in[i] - v[i]);
+    sum[i] = all[i];
   }
 }
 
@@ -110,9 +122,11 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
   int* s_new = s_row + p.B + 1;          // [B + 1]
   int* s_item = s_new + p.B + 1;         // [B + 1]
   unsigned* s_used = reinterpret_cast<unsigned*>(s_item + p.B + 1);  // [slots / 32]
-  __shared__ int s_bad, part[kPlanThreads / 64][3];
+  __shared__ int s_bad;
+  __shared__ int4 part[kPlanThreads / 64];
   const int tid = threadIdx.x, nt = blockDim.x, page = 1 << p.k;
   for (int i = tid; i < (p.slots + 31) / 32; i += nt) s_used[i] = 0;
+  if (tid < kPlanThreads / 64) part[tid] = make_int4(0, 0, 0, 0);
   if (tid == 0) s_bad = 0;
   int nfree = *p.nfree;
   __syncthreads();
@@ -213,9 +227,11 @@ __global__ __launch_bounds__(kPlanThreads) void pages_release_kernel(ReleasePara
   extern __shared__ int lds[];
   int* s_new = lds;  // [B + 1]
   unsigned* s_used = reinterpret_cast<unsigned*>(s_new + p.B + 1);
-  __shared__ int s_bad, part[kPlanThreads / 64][3];
+  __shared__ int s_bad;
+  __shared__ int4 part[kPlanThreads / 64];
   const int tid = threadIdx.x, nt = blockDim.x, page = 1 << p.k;
   for (int i = tid; i < (p.slots + 31) / 32; i += nt) s_used[i] = 0;
+  if (tid < kPlanThreads / 64) part[tid] = make_int4(0, 0, 0, 0);
   if (tid == 0) s_bad = 0;
   const int nfree = *p.nfree;
   __syncthreads();
@@ -281,8 +297,8 @@ int llj_pages_extend(const int* slot, const int* add, int B, int* seen, int slot
   const int most = M > p.nwork ? M : p.nwork, here = most <= kFewRows;
   const size_t lds = ((size_t)3 * (B + 1) + (slots + 31) / 32) * 4;
   hipStream_t s = (hipStream_t)stream;
-  // few sequences and rows: fewer waves to start and to wait for at the barriers
-  const int want = B > M ? B : here ? most : B, nt = want <= 64 ? 64 : want <= 256 ? 256 : kPlanThreads;
+  // few sequences, pages and rows: fewer waves to start and to wait for at the barriers
+  const int work_here = here ? most : M >> k, want = B > work_here ? B : work_here, nt = want <= 64 ? 64 : want <= 256 ? 256 : kPlanThreads;
   hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(nt), lds, s, p, here);
   if (!here) hipLaunchKernelGGL(pages_rows_kernel, dim3((most + 255) / 256), dim3(256), 0, s, p);
   LLJ_CHECK_LAUNCH();

@@ -14,8 +14,15 @@ import torch
 from . import _hip
 from .pages import PAGE_SIZES, ints, on_device
 
-WGS = 512  # workgroups that the keys of a call are split for
-RANGE = 256  # the shortest key range
+# Key ranges of a call, at most. Few rows: a range is at least a round of its workgroup's waves, from 16 ranges on two (one sequence of 16,000 keys, 8
+# K / V heads: 32 ranges 15.0 us, 63 18.3; of 4,000: 16 ranges 10.5, 8 11.1), and 512 workgroups fill the GPU (8 sequences of 4,000: 8 ranges
+# 15.0 us, 4 16.0, 16 19.7). A sequence that is shorter than the table allows takes fewer by itself. Prompt rows, whose ranges are
+# put together by a launch of their own: 1,024 keys (512 rows behind 60,000 tokens: 4 ranges 703 us, one 1,925; 512 rows of a
+# prompt alone: one 25.9, two 28.4).
+WGS = 512
+RANGE, RANGES = 256, 16
+PROMPT_RANGE = 1024
+FEW_COLUMNS = 64  # (row, head) pairs of a K / V head in an item: from more on it is prompt rows (csrc/kv4_attend.hip)
 
 
 def _dt(t: torch.dtype) -> int:
@@ -113,7 +120,22 @@ def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: 
     tiles = _hip.lib().llj_kv4_tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
     if not tiles:
         raise ValueError(f"{heads} heads on {layout.kv_heads}, items of {rows} rows")
-    return max(1, min(64, -(-keys // RANGE), WGS // max(1, items * tiles))), items * tiles
+    if rows * heads // layout.kv_heads > FEW_COLUMNS:
+        n = -(-keys // PROMPT_RANGE)
+    else:
+        n = -(-keys // RANGE)
+        if n > RANGES:
+            n = max(RANGES, -(-keys // (2 * RANGE)))
+    return max(1, min(64, n, WGS // max(1, items * tiles))), items * tiles
+
+
+def item_rows(layout: Layout, heads: int, longest: int, dtype: torch.dtype) -> int:
+    """Rows of a work item for sequences of up to `longest` rows in a call: few rows share the 16 columns of a tile, prompt rows the
+    128 (fp32 rows and heads over 128: 64) that a tile of keys is unpacked for."""
+    R = heads // layout.kv_heads
+    if longest * R <= FEW_COLUMNS:
+        return max(1, 16 // R)
+    return max(1, (128 if dtype == torch.bfloat16 and max(layout.dim, layout.vdim) <= 128 else 64) // R)
 
 
 def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Tensor, slot: torch.Tensor, pos: torch.Tensor, *,
