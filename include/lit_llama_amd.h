@@ -619,7 +619,7 @@ int llj_streams_linear(int act, const void* y, const float* out_w, const float* 
  * values ov, one gate per head at og (-1: none).
  * prep: rotate-half rotation of the first rot_dims dimensions of queries (in place) and keys (turns[i] = frequency of pair
  * (i, i + rot_dims / 2) / 2 pi, doubles), with qk_norm both divided by their root mean square over dim; key and value
- * into the cache. first (row stride ldf): without lam a copy of the values is left there, with lam the values are
+ * into the cache (W 0: row m's into row m of it). first (row stride ldf): without lam a copy of the values is left there, with lam the values are
  * (1 - lam) v + lam first.
  * rows: any sizes; softmax over the row's own and all earlier positions of q . k * scale, with sink one added to the
  * denominator; y = sum p v * sigmoid(gate).

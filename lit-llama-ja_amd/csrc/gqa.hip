@@ -27,7 +27,7 @@ struct GqaParams {
   const int* pos;      // position of each row
   const int* row_seq;  // NULL: row m is sequence m
   const int* slot;
-  void* cache;  // [slots][W][ldc]
+  void* cache;  // [slots][W][ldc]; W 0 (preparation only): [M][ldc]
   int W, ldc;
   void* first;  // [M][ldf]
   const float* lam;
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void gqa_prep_kernel(GqaParams p, int LG) {
   const int m = blockIdx.x, tid = threadIdx.x, n = p.RD / 2, D = p.D;
   T* row = (T*)p.in + (size_t)m * p.ld;
   const int ps = p.pos[m], b = p.row_seq ? p.row_seq[m] : m;
-  T* dst = (T*)p.cache + ((size_t)p.slot[b] * p.W + ps) * p.ldc;
+  T* dst = (T*)p.cache + (p.W ? (size_t)p.slot[b] * p.W + ps : (size_t)m) * p.ldc;
   for (int i = tid; i < n; i += 256) turn_cs(p.turns[i], ps, s_cs[i], s_cs[n + i]);
   __syncthreads();
   const int l = tid & (LG - 1), per = 256 / LG;
@@ -692,8 +692,8 @@ __global__ __launch_bounds__(256) void gqa_attend_kernel(GqaParams p, float* par
   }
 }
 
-static int gqa_check(const GqaParams& p) {
-  LLJ_REQUIRE(p.in && p.pos && p.slot && p.cache && p.W > 0 && p.M > 0 && p.H > 0 && p.G > 0 && p.H % p.G == 0 && p.D > 0 &&
+static int gqa_check(const GqaParams& p, int least = 1) {
+  LLJ_REQUIRE(p.in && p.pos && p.slot && p.cache && p.W >= least && p.M > 0 && p.H > 0 && p.G > 0 && p.H % p.G == 0 && p.D > 0 &&
               p.V > 0 && p.ldc >= p.G * (p.D + p.V) && p.oq >= 0 && p.oq + p.H * p.D <= p.ld &&
               (p.og < 0 || p.og + p.H <= p.ld));
   return 0;
@@ -776,7 +776,7 @@ int llj_gqa_prep(void* in, int ld, int oq, int ok, int ov, const void* turns, in
   p.pos = pos; p.row_seq = row_seq; p.slot = slot; p.cache = cache; p.W = W; p.ldc = ldc;
   p.first = first; p.lam = lam; p.ldf = ldf; p.M = M; p.H = heads; p.G = kv_heads; p.D = dim; p.V = vdim;
   LLJ_REQUIRE(dt == 0 || dt == 1);
-  if (const int rc = gqa_check(p)) return rc;
+  if (const int rc = gqa_check(p, 0)) return rc;
   if (const int rc = gqa_check_new(p)) return rc;
   const size_t lds = (size_t)(rot_dims > 0 ? rot_dims : 2) * 4;
   LLJ_REQUIRE(lds <= 64 * 1024);

@@ -34,12 +34,14 @@ EOS_CHECK_EVERY = 16  # greedy graph path: host looks at the ids once per 16 tok
 
 @torch.no_grad()
 def generate(model: LLaMA, idx: torch.Tensor, max_new_tokens: int, *, max_seq_length: Optional[int] = None,
-             temperature: float = 1.0, top_k: Optional[int] = None, eos_id: Optional[int] = None) -> torch.Tensor:
+             temperature: float = 1.0, top_k: Optional[int] = None, eos_id: Optional[int] = None,
+             kv_cache: Optional[str] = None) -> torch.Tensor:
     """Takes a conditioning sequence (prompt) as input and continues to generate as many tokens as requested.
 
     Reference generate.py:18-89. Every decode step, greedy (top_k=1) or sampled, is one replay of
     the captured HIP graph; sampling draws its uniforms from a counter hash seeded from torch's
-    default generator, so torch.manual_seed makes a run reproducible as in the reference."""
+    default generator, so torch.manual_seed makes a run reproducible as in the reference. kv_cache "int4" (models with
+    per-sequence state): keys and values in 4 bits."""
     T = idx.size(0)
     T_new = T + max_new_tokens
     if max_seq_length is None:
@@ -47,7 +49,12 @@ def generate(model: LLaMA, idx: torch.Tensor, max_new_tokens: int, *, max_seq_le
     if max_new_tokens <= 0:
         return idx.clone()
     seed = 0 if top_k == 1 else int(torch.randint(0, 2 ** 62, (1,)))
-    sess = DecodeSession(model, 1, max_seq_length, T_new, temperature=temperature, top_k=top_k, seed=seed)
+    state = None
+    if kv_cache is not None:
+        if not hasattr(model, "new_state"):
+            raise ValueError("this model keeps its keys and values in its own type")
+        state = model.new_state(1, max_seq_length, kv_cache)
+    sess = DecodeSession(model, 1, max_seq_length, T_new, temperature=temperature, top_k=top_k, seed=seed, state=state)
     return _run_session(sess, idx, max_new_tokens, eos_id)
 
 
@@ -101,11 +108,11 @@ def generate_batch(model: LLaMA, idx: torch.Tensor, max_new_tokens: int, *, max_
 def main(prompt: str = "Hello, my name is", *, num_samples: int = 1, max_new_tokens: int = 50, top_k: int = 200,
          temperature: float = 0.8, checkpoint_path: Path = Path("checkpoints/lit-llama/7B/lit-llama.pth"),
          tokenizer_path: Path = Path("checkpoints/lit-llama/tokenizer.model"), quantize: Optional[str] = None,
-         prompt_tokens: Optional[List[int]] = None, dtype: str = "bfloat16") -> None:
+         prompt_tokens: Optional[List[int]] = None, dtype: str = "bfloat16", kv_cache: Optional[str] = None) -> None:
     """Generates text samples based on a pre-trained LLaMA model and tokenizer (reference generate.py:92-155).
 
     checkpoint_path may be a model folder (config.json + model.safetensors) of any registered architecture,
-    with `dtype` its weights' and activations' type. With prompt_tokens (ids) no tokenizer is read and the
+    with `dtype` its weights' and activations' type, and `kv_cache` "int4" its keys and values in 4 bits. With prompt_tokens (ids) no tokenizer is read and the
     samples are printed as ids."""
     folder = is_model_folder(checkpoint_path)
     assert folder or checkpoint_path.is_file(), checkpoint_path
@@ -113,6 +120,8 @@ def main(prompt: str = "Hello, my name is", *, num_samples: int = 1, max_new_tok
         raise SystemExit("--quantize takes lit-llama checkpoint files, not model folders")
     if not folder and dtype != "bfloat16":
         raise SystemExit("--dtype is for model folders; checkpoint files run in bfloat16")
+    if not folder and kv_cache is not None:
+        raise SystemExit("--kv_cache is for model folders")
     assert prompt_tokens is not None or tokenizer_path.is_file(), tokenizer_path
     if not torch.cuda.is_available():
         raise SystemExit("this generate.py runs on a ROCm GPU (MI355X) only")
@@ -139,7 +148,7 @@ def main(prompt: str = "Hello, my name is", *, num_samples: int = 1, max_new_tok
     for i in range(num_samples):
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        y = generate(model, encoded, max_new_tokens, temperature=temperature, top_k=top_k)
+        y = generate(model, encoded, max_new_tokens, temperature=temperature, top_k=top_k, kv_cache=kv_cache)
         torch.cuda.synchronize()
         t = time.perf_counter() - t0
         model.reset_cache()
@@ -163,7 +172,8 @@ if __name__ == "__main__":
                     help="token ids instead of --prompt (no tokenizer; ids are printed)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"],
                     help="of a model folder (--checkpoint_path naming one)")
+    ap.add_argument("--kv_cache", default=None, choices=[None, "int4"], help="of a model folder: keys and values in 4 bits")
     a = ap.parse_args()
     main(a.prompt, num_samples=a.num_samples, max_new_tokens=a.max_new_tokens, top_k=a.top_k,
          temperature=a.temperature, checkpoint_path=a.checkpoint_path, tokenizer_path=a.tokenizer_path,
-         quantize=a.quantize, prompt_tokens=a.prompt_tokens, dtype=a.dtype)
+         quantize=a.quantize, prompt_tokens=a.prompt_tokens, dtype=a.dtype, kv_cache=a.kv_cache)

@@ -107,7 +107,7 @@ class _Work(Scratch):
 
 @register("Bobasun")
 class Bobasun(HybridModel):
-    HIP_SOURCES = ("streams", "post_gemv", "gemm_bf16", "gqa", "generic", "ops", "options")
+    HIP_SOURCES = ("streams", "post_gemv", "gemm_bf16", "gqa", "generic", "ops", "options", "pages", "kv4", "kv4_attend", "kv4_flash")
 
     def __init__(self, config: BobasunConfig):
         super().__init__()
@@ -203,6 +203,8 @@ class Bobasun(HybridModel):
         product closes it, in its own launch for one row (PackedLinear.apply_streams) or in one before it."""
         c, M, C, eps, S, dt = self.config, rows.M, self.config.n_embd, self.config.eps, self.config.streams, _dt(self.dtype)
         x, done = w.x, None
+        if state.cache is not None:
+            rows.pages = state.extend(rows)
         first = self.subs[0][0]
         _hip.call("llj_streams_embed", rows.tok.data_ptr(), self.embed.data_ptr(), C, c.embed_scale,
                   rows.pos.data_ptr() if rows.decode else None, x.data_ptr(), C, S, first.inp.data_ptr(), first.norm.data_ptr(),

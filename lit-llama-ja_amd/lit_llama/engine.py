@@ -232,8 +232,12 @@ class HybridProgram(_Program):
 
     def room(self, n: int) -> None:
         """State for n more tokens per row."""
-        if self.state.ensure(max(self.seen) + n):
+        if self.state.room(self.slots, [k + n for k in self.seen]):
             self.sess._drop_graph()
+
+    def check(self) -> None:
+        if getattr(self.state, "cache", None) is not None:
+            self.state.check()
 
     def finish(self, live: list) -> None:
         kept = set(live)

@@ -96,8 +96,9 @@ class HybridModel(torch.nn.Module):
     def act_dtype(self) -> torch.dtype:
         return self.dtype
 
-    def new_state(self, slots: int, max_length: Optional[int] = None) -> SequenceState:
-        return SequenceState(self, slots, max_length)
+    def new_state(self, slots: int, max_length: Optional[int] = None, cache: Optional[str] = None) -> SequenceState:
+        """State of `slots` sequences; cache "int4": the keys and values of full-attention layers in 4 bits."""
+        return SequenceState(self, slots, max_length, cache)
 
     def check_tokens(self, tokens) -> None:
         if len(tokens) and not 0 <= min(tokens) <= max(tokens) < self.config.vocab_size:
@@ -121,7 +122,7 @@ class HybridModel(torch.nn.Module):
                 idx += [base + k for k in ks]
                 base += len(t)
             pick, n = torch.tensor(idx, dtype=torch.int32).to(self.device), len(idx)
-        state.ensure(max(s + len(t) for s, t in zip(starts, tokens)))
+        state.room(slots, [s + len(t) for s, t in zip(starts, tokens)])
         logits = torch.empty(n, self.head.Np, dtype=self.dtype, device=self.device)
         self.run(rows, self.new_work(rows.M), state, logits, pick, _hip.stream(), taps)
         return logits[:, :self.config.vocab_size]

@@ -5,7 +5,8 @@
   * every latent-attention layer's ring of the last tokens' latents, one per layer that projects its own
     (layers that read another layer's latents have none), sized by the widest window among its readers,
   * every full-attention layer's K / V rows, the same buffers with a row for every position: as many as the
-    longest sequence allowed, or without a limit as many as the longest has needed so far (`ensure`),
+    longest sequence allowed, or without a limit as many as the longest has needed so far (`ensure`); or, with cache="int4", the
+    layers' rows in 4 bits in pages that sequences take as they grow (kv4, pages: one block table for all layers),
   * the previous token of each sequence (models whose embedding looks back one token).
 A sequence holds a slot from `alloc` to `release`; kernels address everything through the slot number, so
 the rows of a batch need not be neighbours in memory and a batch can shrink without moving state.
@@ -14,14 +15,20 @@ from __future__ import annotations
 
 import torch
 
+from . import kv4, pages
+
 ALL_POSITIONS = -1  # mixer.ring_window() of layers that keep every token
 GROW_ROWS = 256  # unlimited layers grow by multiples of this many rows
+PAGE = 64  # tokens of a page
 
 
 class SequenceState:
-    def __init__(self, model, slots: int, max_length: int | None = None):
-        """max_length: no sequence will be longer (rings are capped at it); None: unbounded."""
-        self.model, self.max_length = model, max_length
+    def __init__(self, model, slots: int, max_length: int | None = None, cache: str | None = None):
+        """max_length: no sequence will be longer (rings are capped at it); None: unbounded. cache: "int4" keeps the rows of
+        full-attention layers in 4 bits (None: in the model's type)."""
+        if cache not in (None, "int4"):
+            raise ValueError(f"cache {cache!r}: None or 'int4'")
+        self.model, self.max_length, self.cache = model, max_length, cache
         self.slots = 0
         self.recurrent: dict = {}
         self.ring: dict = {}
@@ -33,6 +40,15 @@ class SequenceState:
             elif w is not None:
                 self.ring_rows[i] = w if max_length is None else max(1, min(w, max_length))
         self._all = [i for i, mixer in enumerate(model.mixers) if mixer.ring_window() == ALL_POSITIONS]
+        self.layout: dict = {}
+        self.pool: dict = {}
+        if cache is not None:
+            if not self._all:
+                raise ValueError("this model has no layers that keep every token: no cache to hold in 4 bits")
+            for i in self._all:
+                del self.ring_rows[i]
+                self.layout[i] = model.mixers[i].cache_layout(PAGE)
+                self.layout[i].block_bytes()  # (sizes that the cache does not take are an error here)
         self._free: list = []
         self._grow(slots)
 
@@ -44,9 +60,52 @@ class SequenceState:
                 self.recurrent[i] = torch.zeros(slots, *shape, dtype=torch.float32, device=dev)
             if i in self.ring_rows:
                 self.ring[i] = torch.zeros(slots, self.ring_rows[i], mixer.cache_width(m.dtype), dtype=m.dtype, device=dev)
+        if self.cache is not None:
+            self._pages = [0] * slots  # pages kept for each sequence: of as many tokens as `room` was asked for
+            width = 1 if self.max_length is None else max(1, -(-self.max_length // PAGE))
+            self.table = torch.full((slots, width), -1, dtype=torch.int32, device=dev)
+            self.seen = torch.zeros(slots, dtype=torch.int32, device=dev)
+            self.free = torch.arange(slots, dtype=torch.int32, device=dev)
+            self.nfree = torch.full((1,), slots, dtype=torch.int32, device=dev)
+            self.fault = torch.zeros(1, dtype=torch.int32, device=dev)
+            self.pool = {i: layout.pool(slots, dev) for i, layout in self.layout.items()}
         self.prev = torch.full((slots,), -1, dtype=torch.int32, device=dev)
         self._free = list(range(slots))
         self.slots = slots
+
+    def room(self, slots: list, lengths: list) -> bool:
+        """Room for the sequences in these slots up to so many tokens each; True if something moved (a captured step must be captured
+        again)."""
+        if self.cache is None:
+            return self.ensure(max(lengths))
+        if self.max_length is not None and max(lengths) > self.max_length:
+            raise ValueError(f"sequence of {max(lengths)} tokens in a state for {self.max_length}")
+        for s, n in zip(slots, lengths):
+            self._pages[s] = max(self._pages[s], -(-n // PAGE))
+        moved, width = False, max(self._pages)
+        if width > self.table.shape[1]:
+            table = torch.full((self.slots, max(width, 2 * self.table.shape[1])), -1, dtype=torch.int32, device=self.table.device)
+            table[:, :self.table.shape[1]] = self.table
+            self.table, moved = table, True
+        have, need = self.free.numel(), sum(self._pages)
+        if need > have:
+            n = max(need, have + have // 2)
+            free = torch.zeros(n, dtype=torch.int32, device=self.free.device)
+            free[:have] = self.free
+            new = torch.arange(have, n, dtype=torch.int32, device=self.free.device)
+            free.index_copy_(0, (self.nfree + new - have).long(), new)  # onto the stack, whose height only the device knows
+            self.free = free
+            self.nfree += n - have
+            for i, old in self.pool.items():
+                self.pool[i] = self.layout[i].pool(n, old.device)
+                self.pool[i][:have] = old
+            moved = True
+        return moved
+
+    def extend(self, rows: "Rows") -> pages.PageRows:
+        """Places in the pages for a call's rows (one block table for all layers), once a call."""
+        add = None if rows.decode else rows.new_tokens()
+        return pages.extend(self.table, self.seen, self.free, self.nfree, rows.slot, add, rows.M, PAGE, fault=self.fault)
 
     def ensure(self, length: int) -> bool:
         """Room for sequences of `length` tokens in the layers that keep every token; True if they moved (a captured
@@ -83,13 +142,26 @@ class SequenceState:
         return out
 
     def release(self, slots) -> None:
-        for s in slots:
-            if s in self._free or not 0 <= s < self.slots:
+        slots = list(slots)
+        for k, s in enumerate(slots):
+            if s in self._free or not 0 <= s < self.slots or s in slots[:k]:
                 raise ValueError(f"slot {s} is not in use")
+        if self.cache is not None:
+            for k in range(0, len(slots), pages.MAX_SEQUENCES):
+                ids = torch.tensor(slots[k:k + pages.MAX_SEQUENCES], dtype=torch.int32, device=self.table.device)
+                pages.release(self.table, self.seen, self.free, self.nfree, ids, PAGE, self.fault)
+            for s in slots:
+                self._pages[s] = 0
         self._free.extend(slots)  # a freed slot is used again after every other free one
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in [*self.recurrent.values(), *self.ring.values(), self.prev])
+        own = [self.table, self.seen, self.free] if self.cache is not None else []
+        return sum(t.numel() * t.element_size() for t in [*self.recurrent.values(), *self.ring.values(), *self.pool.values(), *own, self.prev])
+
+    def check(self) -> None:
+        """Waits for the calls so far and raises if one of them found no place for its rows."""
+        if self.cache is not None and int(self.fault):
+            raise RuntimeError("a call's rows found no pages: this state's sequences are not valid")
 
 
 class Rows:
@@ -131,6 +203,10 @@ class Rows:
 
     def _device(self, values: list) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).to(self.pos.device)
+
+    def new_tokens(self) -> torch.Tensor:
+        """The sequences' numbers of rows, on the device (packed rows)."""
+        return self._table("new", lambda: self._device(self.lengths))
 
     def chunks(self, C: int):
         """Packed rows cut into chunks of at most C tokens of one sequence: (number, table [(first row, rows,
