@@ -53,6 +53,9 @@ __device__ __forceinline__ void split_bf(float a, float b, uint32_t (&o)[N]) {
 }
 template <int N>
 __device__ __forceinline__ void split_h(float a, float b, uint32_t (&o)[N]) {
+  // The terms are of a and b as fp32 numbers. Left to see the products that they are, the compiler rounds those to fp16 a second time,
+  // unrounded, for the remainder: another first term now and then, and the sum off by its last place
+  if constexpr (N > 1) asm volatile("" : "+v"(a), "+v"(b));
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const f16x2 h = {(_Float16)a, (_Float16)b};
