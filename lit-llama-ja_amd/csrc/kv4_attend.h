@@ -67,11 +67,24 @@ __device__ __forceinline__ void split_h(float a, float b, uint32_t (&o)[N]) {
   }
 }
 
+// The masks and bases of the unpacking below in registers the compiler cannot see through: as literals they cost it an and and an or each,
+// masks in scalar and bases in vector registers one and-or
+struct Kv4Codes {
+  uint32_t mask_bf, base_bf, mask_h, base_h;
+};
+__device__ __forceinline__ Kv4Codes kv4_codes() {
+  Kv4Codes c;
+  asm("s_mov_b32 %0, 0x00780078" : "=s"(c.mask_bf));
+  asm("v_mov_b32 %0, 0x41804180" : "=v"(c.base_bf));
+  asm("s_mov_b32 %0, 0x03C003C0" : "=s"(c.mask_h));
+  asm("v_mov_b32 %0, 0x4C004C00" : "=v"(c.base_h));
+  return c;
+}
 // A codes' word as four pairs of values (j, j + 4) in word j: 16 + c as bf16 (bits 3 .. 6 are its units from 16 on) ...
 template <bool EXACT>
-__device__ __forceinline__ u32x4 codes_bf(uint32_t w) {
-  const uint32_t m = 0x00780078u, b = 0x41804180u;
-  u32x4 o = {and_or(w << 3, m, b), and_or(w >> 1, m, b), and_or(w >> 5, m, b), and_or(w >> 9, m, b)};
+__device__ __forceinline__ u32x4 codes_bf(uint32_t w, const Kv4Codes& k) {
+  u32x4 o = {and_or(w << 3, k.mask_bf, k.base_bf), and_or(w >> 1, k.mask_bf, k.base_bf), and_or(w >> 5, k.mask_bf, k.base_bf),
+             and_or(w >> 9, k.mask_bf, k.base_bf)};
   if constexpr (EXACT) {  // c - 8
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -81,9 +94,9 @@ __device__ __forceinline__ u32x4 codes_bf(uint32_t w) {
 }
 // ... or as fp16 (bits 6 .. 9)
 template <bool EXACT>
-__device__ __forceinline__ u32x4 codes_h(uint32_t w) {
-  const uint32_t m = 0x03C003C0u, b = 0x4C004C00u;
-  u32x4 o = {and_or(w << 6, m, b), and_or(w << 2, m, b), and_or(w >> 2, m, b), and_or(w >> 6, m, b)};
+__device__ __forceinline__ u32x4 codes_h(uint32_t w, const Kv4Codes& k) {
+  u32x4 o = {and_or(w << 6, k.mask_h, k.base_h), and_or(w << 2, k.mask_h, k.base_h), and_or(w >> 2, k.mask_h, k.base_h),
+             and_or(w >> 6, k.mask_h, k.base_h)};
   if constexpr (EXACT) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

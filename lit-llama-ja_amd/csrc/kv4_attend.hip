@@ -4,16 +4,36 @@
 // and the rows of a short item share its bytes. Waves walk 16 NB keys at a time on their own (no barriers). K fragment: lane (r, g) holds words KT g .. KT g + KT - 1 of key r, one load of 4 KT bytes, and the
 // queries are loaded in that order. V fragment: lane (r, g) takes 4 VH columns of 8 keys; two keys' halves are permuted into one word first,
 // so no transposition is needed. A wave's results, then the workgroups', are merged by their maxima.
+// Items of up to 8 or 4 columns leave most of the product's 16 unused, and with them most lanes of the softmax: the columns are then given PACK
+// times, and the copies' lanes take the scores of different 16-key blocks, which they have anyhow. Their weights go back to the first copy by
+// moves inside a row of lanes.
 #include "kv4_attend.h"
 #include "lit_llama_amd.h"
 
 namespace llj {
 
-template <typename T, int KT, int VH>
+constexpr int kv4_step_blocks(int KT, int VH) { return KT <= 4 && VH <= 2 ? 4 : 2; }
+
+// f over the copies of a column, the result in every copy; and a word of copy b for the first copy
+template <int PACK, typename F>
+__device__ __forceinline__ float over_banks(float v, F f) {
+  if constexpr (PACK >= 2) v = f(v, dpp_f32<0x128>(v));  // the lane 8 further round its row
+  if constexpr (PACK >= 4) v = f(v, dpp_f32<0x124>(v));
+  return v;
+}
+template <int PACK>
+__device__ __forceinline__ uint32_t from_bank(uint32_t v, int b) {  // (b: a constant once the loops are unrolled)
+  if (PACK == 2) return b ? dpp_u32<0x108>(v) : v;
+  if (PACK == 4) return b == 1 ? dpp_u32<0x104>(v) : b == 2 ? dpp_u32<0x108>(v) : b == 3 ? dpp_u32<0x10C>(v) : v;
+  return v;
+}
+
+template <typename T, int KT, int VH, int PACK>
 __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_kernel(Kv4Attend p) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 2 : 1;
-  constexpr int NB = KT <= 4 && VH <= 2 ? 4 : 2, STEP = 16 * NB;  // keys a step
+  constexpr int NB = kv4_step_blocks(KT, VH), STEP = 16 * NB;  // keys a step
+  constexpr int NJ = NB / PACK, CW = 16 / PACK;                // blocks of 16 keys to a lane; columns
   constexpr int KB = 16 * KT, VB = 32 * VH;                      // bytes of a key's, a value's codes
   constexpr int VW = 64 * VH, RP = VW + 4;
   constexpr int VD = VH >= 2 ? VH / 2 : 1;  // words of a value in a lane (VH 1: half of one)
@@ -21,7 +41,9 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   extern __shared__ __attribute__((aligned(16))) float red[];  // [4][16][RP], the waves' results; maxima, sums
   float* wm = red + 4 * 16 * RP;
   float* wl = wm + 64;
+  const Kv4Codes codes = kv4_codes();
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
+  const int bank = col / CW;  // the copy of the columns that this lane is in: its blocks are PACK j + bank
   const int R = p.H / p.pool.G, HB = (p.rows * R + 15) / 16;
   const int item = blockIdx.x, gh = blockIdx.y / HB, hb = blockIdx.y % HB, sp = blockIdx.z;
   int r0 = item, n = 1, b = item;
@@ -39,7 +61,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   const bool held = sl >= 0 && sl < p.slots;
   const kv4_row tab = scalar_row(p.table + (size_t)(held ? uniform(sl) : 0) * p.ldt);
   int row, head;
-  cols.at(col < nc ? col : nc - 1, row, head);
+  cols.at(col % CW < nc ? col % CW : nc - 1, row, head);
   const int k = p.pool.k, pmask = (1 << k) - 1;
   // the keys a column sees: positions up to its row's, in the table
   int pc = p.pos[row];
@@ -54,8 +76,9 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   }
   plast = uniform(plast);
   pfirst = uniform(pfirst);
-  // as many ranges as there are rounds of the four waves: what the caller sized for the longest sequence costs a short one nothing
-  const int steps = plast < 0 ? 0 : plast / STEP + 1, rounds = (steps + 3) / 4, ranges = rounds < 1 ? 1 : rounds < p.nsplit ? rounds : p.nsplit;
+  // at most as many ranges as there are rounds of the four waves, and one for two rounds (300 keys: 7.5 us in one, 8.1 in two; 600: 8.8 in
+  // one, 8.1 in three): what the caller sized for the longest sequence costs a short one nothing
+  const int steps = plast < 0 ? 0 : plast / STEP + 1, rounds = (steps + 3) / 4, ranges = rounds <= 2 ? 1 : rounds < p.nsplit ? rounds : p.nsplit;
   if (sp >= ranges) return;
   const int per = (steps + ranges - 1) / ranges;
   const int s0 = sp * per, s1 = s0 + per < steps ? s0 + per : steps;
@@ -68,8 +91,8 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   // ---- a step's codes and pairs. Each is fetched anew right behind its use, for the wave's next step: no copies, and every load has most of a step
   // to arrive. The page numbers are read a step ahead of that.
   uint32_t kw[NB][KT], vw[NB][4][VD];
-  u32x4 kp[NB], vp[NB];
-  const uint8_t* blk[NB];  // blocks of the step being fetched
+  u32x4 kp[NJ], vp[NJ];
+  size_t blk[NB];  // blocks of the step being fetched: their places in the pool
   int off[NB], idn[NB];
   bool ok[NB], okn[NB];
   auto pages = [&](int t) {
@@ -84,13 +107,13 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     for (int j = 0; j < NB; ++j) {
       okn[j] = idn[j] >= 0 && idn[j] < p.pool.pages;
       off[j] = (STEP * t + 16 * j) & pmask;
-      blk[j] = p.pool.p + ((size_t)(okn[j] ? idn[j] : 0) * p.pool.G + gh) * p.pool.blk;
+      blk[j] = ((size_t)(okn[j] ? idn[j] : 0) * p.pool.G + gh) * p.pool.blk;
     }
   };
   auto fetch_keys = [&] {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const uint8_t* ka = blk[j] + (off[j] + col) * KB + 4 * KT * g;
+      const uint8_t* ka = p.pool.p + blk[j] + (off[j] + col) * KB + 4 * KT * g;
       if constexpr (KT == 2) {
         const uint2 x = *reinterpret_cast<const uint2*>(ka);
         kw[j][0] = x.x;
@@ -105,14 +128,29 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
       }
     }
   };
-  auto fetch_pairs = [&](u32x4 (&o)[NB], int at) {
+  auto pick = [&](auto of, int j) {  // of(PACK j + bank): all of them, then a selection (selected first, they are indexed in memory)
+    const auto a = of(PACK * j);
+    if constexpr (PACK == 1) {
+      return a;
+    } else {
+      const auto b = of(PACK * j + 1);
+      const auto lo = bank & 1 ? b : a;
+      if constexpr (PACK == 2) {
+        return lo;
+      } else {
+        const auto c = of(2), d = of(3), hi = bank & 1 ? d : c;
+        return bank & 2 ? hi : lo;
+      }
+    }
+  };
+  auto fetch_pairs = [&](u32x4 (&o)[NJ], int at) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) o[j] = *reinterpret_cast<const u32x4*>(blk[j] + at + 4 * (off[j] + 4 * g));
+    for (int j = 0; j < NJ; ++j) o[j] = *reinterpret_cast<const u32x4*>(p.pool.p + pick([&](int b) { return blk[b] + 4 * off[b]; }, j) + (at + 16 * g));
   };
   auto fetch_values = [&] {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const uint8_t* va = blk[j] + p.pool.vc + (off[j] + 4 * g) * VB + 2 * VH * col;
+      const uint8_t* va = p.pool.p + blk[j] + p.pool.vc + (off[j] + 4 * g) * VB + 2 * VH * col;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (VH == 1) {
@@ -164,46 +202,49 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
       s[j] = begin;
 #pragma unroll
       for (int kk = 0; kk < KT; ++kk) {
-        const bf16x8 a = __builtin_bit_cast(bf16x8, codes_bf<F32>(kw[j][kk]));
+        const bf16x8 a = __builtin_bit_cast(bf16x8, codes_bf<F32>(kw[j][kk], codes));
 #pragma unroll
         for (int i = 0; i < NQ; ++i) s[j] = mfma_bf16(a, __builtin_bit_cast(bf16x8, qf[i][kk]), s[j]);
       }
     }
     fetch_keys();
+    f32x4 sm[NJ];  // keys STEP t + 16 (PACK j + bank) + 4 g + i
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      f32x4 sc, of;
+    for (int j = 0; j < NJ; ++j) {
+      f32x4 sc, of, x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        x[i] = pick([&](int b) { return (float)s[b][i]; }, j);
         sc[i] = bflo(kp[j][i]);
         of[i] = F32 ? bfhi(kp[j][i]) + 8.f * sc[i] : bfhi(kp[j][i]);
       }
-      s[j] = kv4_scores(s[j], sc, of, qs);
+      sm[j] = kv4_scores(x, sc, of, qs);
     }
     fetch_pairs(kp, p.pool.ks);
     const bool masked = gap || STEP * t + STEP - 1 > pfirst;  // (uniform)
     if (masked) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
-        const int lim = ok[j] ? pc : -1;
+      for (int j = 0; j < NJ; ++j) {
+        const int lim = pick([&](int b) { return ok[b] ? pc : -1; }, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (STEP * t + 16 * j + 4 * g + i > lim) {
-            s[j][i] = -INFINITY;
+          if (STEP * t + 16 * (PACK * j + bank) + 4 * g + i > lim) {
+            sm[j][i] = -INFINITY;
             vp[j][i] = 0;  // (what stands behind a sequence's end is never multiplied in)
           }
       }
     }
     float mx = -INFINITY, ms = kScaleMin;
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mx = fmaxf(mx, s[j][i]);
+        mx = fmaxf(mx, sm[j][i]);
         ms = fmaxf(ms, bflo(vp[j][i]));
       }
+    mx = over_banks<PACK>(mx, [](float a, float b) { return fmaxf(a, b); });
     mx = groups_max(mx);
-    ms = groups_max(masked ? row16_max(ms) : ms);
+    ms = groups_max(masked || PACK > 1 ? row16_max(ms) : ms);
     if (__any(mx > m_run + slack) || ms > unit + unit) {  // (uniform) a new maximum, or larger scales
       const float m_new = fmaxf(m_run, mx), grown = fmaxf(unit, pow2_floor(ms));
       float corr = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * sl2);
@@ -220,22 +261,26 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
         for (int i = 0; i < 4; ++i) acc[d][i] *= corr;
     }
     const float mu = m_run == -INFINITY ? 0.f : m_run, mus = mu * sl2;
-    uint32_t pt[NB][2][NP];
+    uint32_t pm[NJ][2][NP], pt[NB][2][NP];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = kv4_weight<F32>(s[j][i], mu, mus, sl2);
+        const float e = kv4_weight<F32>(sm[j][i], mu, mus, sl2);
         l_run += e;
         z_run = fmaf(e, bfhi(vp[j][i]), z_run);
         w[i] = e * (bflo(vp[j][i]) * up);
         if (F32) b_run += w[i];
       }
-      split_h<NP>(w[0], w[1], pt[j][0]);
-      split_h<NP>(w[2], w[3], pt[j][1]);
-      if (!F32) b_run = add_pair(pt[j][1][0], add_pair(pt[j][0][0], b_run));
+      split_h<NP>(w[0], w[1], pm[j][0]);
+      split_h<NP>(w[2], w[3], pm[j][1]);
+      if (!F32) b_run = add_pair(pm[j][1][0], add_pair(pm[j][0][0], b_run));
     }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)  // block j's weights to the first copy of the columns (the others' columns are never stored)
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) pt[j][i / NP][i % NP] = from_bank<PACK>(pm[j / PACK][i / NP][i % NP], j % PACK);
     fetch_pairs(vp, p.pool.vs);
 #pragma unroll
     for (int u = 0; u < NB / 2; ++u)
@@ -245,7 +290,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
 #pragma unroll
         for (int e = 0; e < 4; ++e) {  // two keys' halves in a word
           const uint32_t a = vw[2 * u + (e >> 1)][2 * (e & 1)][v / 2], c = vw[2 * u + (e >> 1)][2 * (e & 1) + 1][v / 2];
-          const u32x4 y = codes_h<F32>(VH == 1 ? a | c << 16 : __builtin_amdgcn_perm(c, a, v % 2 ? 0x07060302u : 0x05040100u));
+          const u32x4 y = codes_h<F32>(VH == 1 ? a | c << 16 : __builtin_amdgcn_perm(c, a, v % 2 ? 0x07060302u : 0x05040100u), codes);
 #pragma unroll
           for (int d = 0; d < 4; ++d) x[d][e] = y[d];
         }
@@ -258,7 +303,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     fetch_values();
     if (!F32 && --fold == 0) {
       fold = kFold;
-      const float z = -BIAS * groups_sum(b_run);
+      const float z = -BIAS * groups_sum(over_banks<PACK>(b_run, [](float a, float b) { return a + b; }));
       b_run = 0.f;
 #pragma unroll
       for (int d = 0; d < 4 * VH; ++d)
@@ -267,9 +312,10 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     }
   }
   // ---- the four waves' results, in order. Lane (col, g) holds values VW / 4 g + 4 VH i + d of its column, d = 4 v + e
-  l_run = groups_sum(l_run);
+  const auto plus = [](float a, float b) { return a + b; };
+  l_run = groups_sum(over_banks<PACK>(l_run, plus));
   const float down = unit * kUnweight;
-  z_run = groups_sum(z_run - BIAS * down * b_run);
+  z_run = groups_sum(over_banks<PACK>(z_run - BIAS * down * b_run, plus));
   {
     float* o = red + (wave * 16 + col) * RP + VW / 4 * g;
 #pragma unroll
@@ -310,9 +356,9 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
   if (ranges > 1) kv4_merge<T, VW>(p, cols, ranges, p.count + (size_t)item * gridDim.y + blockIdx.y, red);
 }
 
-template <typename T, int KT, int VH>
+template <typename T, int KT, int VH, int PACK>
 static int kv4_attend_go(const Kv4Attend& p, hipStream_t s) {
-  auto kern = kv4_attend_kernel<T, KT, VH>;
+  auto kern = kv4_attend_kernel<T, KT, VH, PACK>;
   constexpr size_t lds = (size_t)(4 * 16 * (64 * VH + 4) + 128) * 4;
   if constexpr (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -324,11 +370,19 @@ static int kv4_attend_go(const Kv4Attend& p, hipStream_t s) {
   return 0;
 }
 
+template <typename T, int KT, int VH>
+static int kv4_attend_pack(const Kv4Attend& p, hipStream_t s) {
+  const int c = p.rows * (p.H / p.pool.G);
+  if constexpr (kv4_step_blocks(KT, VH) == 4)
+    if (c <= 4) return kv4_attend_go<T, KT, VH, 4>(p, s);
+  return c <= 8 ? kv4_attend_go<T, KT, VH, 2>(p, s) : kv4_attend_go<T, KT, VH, 1>(p, s);
+}
+
 template <typename T, int KT>
 static int kv4_attend_values(const Kv4Attend& p, hipStream_t s) {
-  if (p.V <= 64) return kv4_attend_go<T, KT, 1>(p, s);
-  if (p.V <= 128) return kv4_attend_go<T, KT, 2>(p, s);
-  return kv4_attend_go<T, KT, 4>(p, s);
+  if (p.V <= 64) return kv4_attend_pack<T, KT, 1>(p, s);
+  if (p.V <= 128) return kv4_attend_pack<T, KT, 2>(p, s);
+  return kv4_attend_pack<T, KT, 4>(p, s);
 }
 
 template <typename T>

@@ -26,6 +26,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   constexpr int KB = 16 * KT, VB = 32 * VH, VW = 64 * VH, VD = VH >= 2 ? VH / 2 : 1;
   typedef Kv4Tile<KT, VH> Tile;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two tiles
+  const Kv4Codes codes = kv4_codes();
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 15, g = lane >> 4;
   constexpr int CW = 64 * QB;  // columns
   const int R = p.H / p.pool.G, CB = (p.rows * R + CW - 1) / CW, x = p.items * CB - 1 - blockIdx.x / p.pool.G;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   };
   auto unpack = [&](uint8_t* buf) {
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) *reinterpret_cast<u32x4*>(buf + (kk * 4 + wave) * 1024 + lane * 16) = codes_bf<F32>(kw[kk]);
+    for (int kk = 0; kk < KT; ++kk) *reinterpret_cast<u32x4*>(buf + (kk * 4 + wave) * 1024 + lane * 16) = codes_bf<F32>(kw[kk], codes);
     uint8_t* vb = buf + Tile::kKeys + (wave >> 1) * 4 * VH * 1024 + lane * 16 + 8 * (wave & 1);
 #pragma unroll
     for (int v = 0; v < VH; ++v) {
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
         if constexpr (VH == 1) x[e] = vw[2 * e][0] | vw[2 * e + 1][0] << 16;
         else x[e] = __builtin_amdgcn_perm(vw[2 * e + 1][v / 2], vw[2 * e][v / 2], v % 2 ? 0x07060302u : 0x05040100u);
       }
-      const u32x4 a = codes_h<true>(x[0]), c = codes_h<true>(x[1]);
+      const u32x4 a = codes_h<true>(x[0], codes), c = codes_h<true>(x[1], codes);
 #pragma unroll
       for (int d = 0; d < 4; ++d) *reinterpret_cast<uint2*>(vb + (4 * v + d) * 1024) = make_uint2(a[d], c[d]);
     }

@@ -15,13 +15,12 @@ from . import _hip
 from .pages import PAGE_SIZES, ints, on_device
 
 # Key ranges of a call, at most. Few rows: a range is at least a round of its workgroup's waves, from 16 ranges on two (one sequence of 16,000 keys, 8
-# K / V heads: 32 ranges 15.0 us, 63 18.3; of 4,000: 16 ranges 10.5, 8 11.1), and 512 workgroups fill the GPU (8 sequences of 4,000: 8 ranges
-# 15.0 us, 4 16.0, 16 19.7). A sequence that is shorter than the table allows takes fewer by itself. Prompt rows, whose ranges are
-# put together by a launch of their own: 1,024 keys (512 rows behind 60,000 tokens: 4 ranges 703 us, one 1,925; 512 rows of a
-# prompt alone: one 25.9, two 28.4).
-WGS = 512
-RANGE, RANGES = 256, 16
-PROMPT_RANGE = 1024
+# K / V heads: 32 ranges 14.2 us, 64 18.0; of 4,000: 16 ranges 10.1, 4 12.7), and 512 workgroups or, of ranges of 1,024 keys, three on a CU (24 sequences
+# of 4,000: 4 ranges 24.5 us, 2 26.4, one 29.5; 32 of 8,000: 3 ranges 49.2, one 54.6; 32 of 2,000: 2 ranges 19.3, one 18.8, 4 21.0). A sequence
+# that is shorter than the table allows takes fewer by itself. Prompt rows, whose ranges are put together by a launch of
+# their own: 1,024 keys (512 rows behind 60,000 tokens: 4 ranges 703 us, one 1,925; 512 rows of a prompt alone: one 25.9, two 28.4).
+WGS, WGS_LONG = 512, 768
+RANGE, RANGES, RANGE_LONG = 256, 16, 1024
 FEW_COLUMNS = 64  # (row, head) pairs of a K / V head in an item: from more on it is prompt rows (csrc/kv4_attend.hip)
 
 
@@ -120,13 +119,15 @@ def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: 
     tiles = _hip.lib().llj_kv4_tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
     if not tiles:
         raise ValueError(f"{heads} heads on {layout.kv_heads}, items of {rows} rows")
+    wgs, long = max(1, items * tiles), -(-keys // RANGE_LONG)
     if rows * heads // layout.kv_heads > FEW_COLUMNS:
-        n = -(-keys // PROMPT_RANGE)
+        n = min(long, WGS // wgs)
     else:
         n = -(-keys // RANGE)
         if n > RANGES:
             n = max(RANGES, -(-keys // (2 * RANGE)))
-    return max(1, min(64, n, WGS // max(1, items * tiles))), items * tiles
+        n = max(min(n, WGS // wgs), min(long, WGS_LONG // wgs))
+    return max(1, min(64, n)), items * tiles
 
 
 def item_rows(layout: Layout, heads: int, longest: int, dtype: torch.dtype) -> int:
