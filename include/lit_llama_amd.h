@@ -681,7 +681,7 @@ int llj_kv4_read(const void* pool, int pages, int page, const int* place, int M,
  * item are left as they are); NULL: row m is sequence m, rows = 1. nsplit <= 64 key ranges; scratch part [M][heads][nsplit]
  * [llj_kv4_part_width(vdim)] fp32 and count [items][llj_kv4_tiles] (0: sizes
  * not taken; the workgroups of an item and range) ints, zero before the first call (a call leaves them zero), for calls of
- * one stream. */
+ * one stream; items of more than 64 (row, head) pairs of a K / V head are prompt rows and take no counters. */
 int llj_kv4_part_width(int vdim);
 int llj_kv4_tiles(int heads, int kv_heads, int dim, int vdim, int rows, int dt);
 int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int* work, int items, int rows, const int* pos, const int* slot, int B,

@@ -414,10 +414,11 @@ int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int*
                    int ldy, int M, int heads, int kv_heads, int dim, int vdim, float scale, int sink, int dt, void* stream) {
   LLJ_REQUIRE(kv4_sizes(pool, pages, page, kv_heads, dim, vdim, dt) && q && pos && slot && table && y && items >= 0 && rows >= 1 && rows <= 65535 &&
               B >= 1 && slots >= 1 && ldt >= 1 && ldt <= (1 << 30) / page && M >= 0 && heads >= 1 && heads % kv_heads == 0 && heads <= 65535 &&
-              ldq >= heads * dim && ldy >= heads * vdim && (!gate || ldg >= heads) && nsplit >= 1 && nsplit <= 64 && (nsplit == 1 || (part && count)) &&
+              ldq >= heads * dim && ldy >= heads * vdim && (!gate || ldg >= heads) && nsplit >= 1 && nsplit <= 64 && (nsplit == 1 || part) &&
               ((uintptr_t)part & 15) == 0 && ((uintptr_t)count & 3) == 0 && (work || (rows == 1 && items <= M && items <= B)));
   const int tiles = llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt);
-  LLJ_REQUIRE(tiles > 0 && (long long)items * tiles <= 0x7fffffff);
+  const bool few = rows * (heads / kv_heads) <= kv4_few_columns;
+  LLJ_REQUIRE(tiles > 0 && (long long)items * tiles <= 0x7fffffff && (nsplit == 1 || !few || count));
   if (items == 0 || M == 0) return 0;
   Kv4Attend p{};
   p.q = q; p.gate = gate; p.ldq = ldq; p.ldg = ldg; p.work = work; p.items = items; p.rows = rows;
@@ -428,7 +429,7 @@ int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int*
   p.part = part; p.count = count; p.nsplit = nsplit;
   p.quads = vdim % 4 == 0 && ldy % 4 == 0 && ((uintptr_t)y & (dt ? 15 : 7)) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (rows * (heads / kv_heads) > kv4_few_columns) return kv4_flash(p, dt, s);
+  if (!few) return kv4_flash(p, dt, s);
   return dt == 0 ? kv4_attend_keys<bf16_t>(p, s) : kv4_attend_keys<float>(p, s);
 }
 

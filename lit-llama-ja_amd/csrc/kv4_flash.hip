@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 
   // ---- a tile's codes: this wave's 16 keys of it
   uint32_t kw[KT], vw[4][VD], pair;
-  bool ok = false;
+  bool ok = false, there = false;
   auto page_of = [&](int t) {
     const int at = (64 * t + 16 * wave) >> k;
     return tab[at < p.ldt ? at : p.ldt - 1];
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
       }
     }
     pair = *reinterpret_cast<const uint32_t*>(blk + (lane & 16 ? p.pool.vs : p.pool.ks) + 4 * (off + col));
-    if (!ok || 64 * t + 16 * wave + col > plast) pair = 0;  // (behind the last row's position stands anything)
+    there = ok && 64 * t + 16 * wave + col <= plast;  // (behind the last row's position stands anything; the pair itself is on its way)
   };
   auto unpack = [&](uint8_t* buf) {
 #pragma unroll
@@ -138,7 +138,8 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
       for (int d = 0; d < 4; ++d) *reinterpret_cast<uint2*>(vb + (4 * v + d) * 1024) = make_uint2(a[d], c[d]);
     }
-    const float sc = bflo(pair), of = bfhi(pair) + (F32 || lane & 16 ? 8.f * sc : 0.f);  // (codes c - 8)
+    const uint32_t so = there ? pair : 0;
+    const float sc = bflo(so), of = bfhi(so) + (F32 || lane & 16 ? 8.f * sc : 0.f);  // (codes c - 8)
     float* at = reinterpret_cast<float*>(buf + Tile::kPairs + (lane & 16) * 32) + wave * 16 + col;  // (lanes 32 .. 63 write the same)
     at[0] = sc;
     at[64] = of;

@@ -79,8 +79,14 @@ def _heads(t: torch.Tensor, what: str, M: int, heads: int, n: int, index: int) -
 
 def _lead(t: torch.Tensor, what: str, M: int, n: int, index: int) -> int:
     """Row stride of rows (M, n) whose values follow one another."""
-    if t.dim() != 2 or t.shape != (M, n) or on_device(t, what) != index:
-        raise ValueError(f"{what} {tuple(t.shape)} on {t.device}: ({M}, {n}) on cuda:{index}")
+    if t.dim() != 2 or t.shape != (M, n):
+        raise ValueError(f"{what} {tuple(t.shape)}: ({M}, {n})")
+    return _stride(t, what, M, n, index)
+
+
+def _stride(t: torch.Tensor, what: str, M: int, n: int, index: int) -> int:
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, the cache on cuda:{index}")
     ld, one = t.stride()
     if M == 1:
         ld = n
@@ -115,19 +121,17 @@ def read(pool: torch.Tensor, layout: Layout, place: torch.Tensor, dtype: torch.d
 
 
 def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[int, int]:
-    """(key ranges, counters) of a call of `items` items of up to `rows` rows over up to `keys` keys."""
+    """(key ranges, counters) of a call of `items` items of up to `rows` rows over up to `keys` keys (prompt rows need no counters)."""
     tiles = _hip.lib().llj_kv4_tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
     if not tiles:
         raise ValueError(f"{heads} heads on {layout.kv_heads}, items of {rows} rows")
     wgs, long = max(1, items * tiles), -(-keys // RANGE_LONG)
     if rows * heads // layout.kv_heads > FEW_COLUMNS:
-        n = min(long, WGS // wgs)
-    else:
-        n = -(-keys // RANGE)
-        if n > RANGES:
-            n = max(RANGES, -(-keys // (2 * RANGE)))
-        n = max(min(n, WGS // wgs), min(long, WGS_LONG // wgs))
-    return max(1, min(64, n)), items * tiles
+        return max(1, min(64, long, WGS // wgs)), 0
+    n = -(-keys // RANGE)
+    if n > RANGES:
+        n = max(RANGES, -(-keys // (2 * RANGE)))
+    return max(1, min(64, max(min(n, WGS // wgs), min(long, WGS_LONG // wgs)))), items * tiles
 
 
 def item_rows(layout: Layout, heads: int, longest: int, dtype: torch.dtype) -> int:
@@ -150,42 +154,44 @@ def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Ten
     key ranges, whose counters `count` a program may keep for all its calls on one stream (int32, zero, `splits` says how many)."""
     index, pages = _pool(pool, layout)
     G, D, V, page = layout.kv_heads, layout.dim, layout.vdim, layout.page
-    if q.dim() != 2 or not q.numel() or q.shape[1] % (G * D):
+    if q.dim() != 2 or not q.numel() or q.size(1) % (G * D):
         raise ValueError(f"q {tuple(q.shape)}: (M, heads {D}) with heads a multiple of {G}")
     M, n = q.shape
-    H, dt, ldq = n // D, _dt(q.dtype), _lead(q, "q", M, n, index)
+    H, dtype = n // D, q.dtype
+    dt, ldq = _dt(dtype), _stride(q, "q", M, n, index)
     ints(table, "table", 2, index)
     slots, width = table.shape
     B = ints(slot, "slot", 1, index)
     if ints(pos, "pos", 1, index) != M:
         raise ValueError(f"{pos.numel()} positions for {M} rows")
     if work is None:
-        items, rows = M, 1
+        items, rows, work_at = M, 1, None
         if B < M:
             raise ValueError(f"{M} rows of {B} sequences without work items")
     else:
-        items = ints(work, "work", 2, index) // 3
-        if work.shape[1] != 3 or rows < 1:
+        items, work_at = ints(work, "work", 2, index) // 3, work.data_ptr()
+        if work.size(1) != 3 or rows < 1:
             raise ValueError("work items are (first row, rows, sequence), of at least one row")
     if out is None:
-        out = torch.empty(M, H * V, dtype=q.dtype, device=q.device)
+        out = torch.empty(M, H * V, dtype=dtype, device=q.device)
         ldo = H * V
     else:
         ldo = _lead(out, "out", M, H * V, index)
-    ldg = 0 if gate is None else _lead(gate, "gate", M, H, index)
-    if out.dtype != q.dtype or (gate is not None and gate.dtype != q.dtype):
-        raise TypeError(f"q, gate and out are of one type, {q.dtype}")
-    n, need = splits(layout, H, items, rows, width * page, q.dtype)
-    part = counters = None
+    gate_at, ldg = (None, 0) if gate is None else (gate.data_ptr(), _lead(gate, "gate", M, H, index))
+    if out.dtype != dtype or (gate is not None and gate.dtype != dtype):
+        raise TypeError(f"q, gate and out are of one type, {dtype}")
+    n, need = splits(layout, H, items, rows, width * page, dtype)
+    part_at = counters = None
     if n > 1:
         part = torch.empty(M * H * n * _hip.lib().llj_kv4_part_width(V), dtype=torch.float32, device=q.device)
-        if count is None:
-            count = torch.zeros(need, dtype=torch.int32, device=q.device)
-        elif ints(count, "count", 1, index) < need:
-            raise ValueError(f"{count.numel()} counters, {need} are needed")
-        counters = count.data_ptr()
-    _hip.call_on(index, "llj_kv4_attend", q.data_ptr(), ldq, None if gate is None else gate.data_ptr(), ldg, None if work is None else work.data_ptr(), items,
-                 rows, pos.data_ptr(), slot.data_ptr(), B, table.data_ptr(), slots, width, pool.data_ptr(), pages, page,
-                 None if part is None else part.data_ptr(), counters, n, out.data_ptr(), ldo, M, H, G, D, V, D ** -0.5 if scale is None else scale,
-                 int(sink), dt)
+        part_at = part.data_ptr()
+        if need:
+            if count is None:
+                count = torch.zeros(need, dtype=torch.int32, device=q.device)
+            elif ints(count, "count", 1, index) < need:
+                raise ValueError(f"{count.numel()} counters, {need} are needed")
+            counters = count.data_ptr()
+    _hip.call_on(index, "llj_kv4_attend", q.data_ptr(), ldq, gate_at, ldg, work_at, items, rows, pos.data_ptr(), slot.data_ptr(), B, table.data_ptr(),
+                 slots, width, pool.data_ptr(), pages, page, part_at, counters, n, out.data_ptr(), ldo, M, H, G, D, V,
+                 D ** -0.5 if scale is None else scale, int(sink), dt)
     return out

@@ -513,7 +513,7 @@ class GroupedAttention:
             n, work, _ = rows.chunks(per)
             work = work.view(n, 3)
         n, need = kv4.splits(layout, s.heads, M if work is None else n, per, state.table.shape[1] * layout.page, self.dtype)
-        count = w.buffer("count4", need, torch.int32, zero=True) if n > 1 else None
+        count = w.buffer("count4", need, torch.int32, zero=True) if n > 1 and need else None
         kv4.attend(p[:M, o[0]:o[0] + s.heads * s.dim], state.pool[i], layout, state.table, rows.slot, rows.pages.pos, work=work, rows=per, scale=s.scale,
                    sink=s.sink, gate=p[:M, o[3]:o[3] + s.heads], out=y[:M, :s.heads * s.vdim], count=count)
 

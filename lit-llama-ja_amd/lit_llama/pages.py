@@ -77,7 +77,8 @@ def _tables(table, seen, free, nfree, slot, page) -> tuple:
 def extend(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: torch.Tensor, slot: torch.Tensor, add: Optional[torch.Tensor],
            M: int, page: int, chunk: int = 0, commit: bool = True, fault: Optional[torch.Tensor] = None) -> PageRows:
     """add[b] more tokens (None: one) for the sequence in slot[b]. M: rows there is room for. commit False: lengths and stack stay as
-    they are (PageRows.seen and .left hold the new ones), and a later call makes the same rows again."""
+    they are (PageRows.seen and .left hold the new ones; the new pages stand in the table already), and a later call makes the same rows
+    again. Calls on one set of tables follow one another on one stream."""
     index, slots, width, B, cap = _tables(table, seen, free, nfree, slot, page)
     if add is not None and ints(add, "add", 1, index) != B:
         raise ValueError(f"{add.numel()} counts for {B} sequences")

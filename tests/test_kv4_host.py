@@ -145,3 +145,24 @@ def test_host_tensors_are_refused():
         kv4.read(pool.int(), lay, i(2))
     with pytest.raises(ValueError):
         kv4.read(lay.pool(3, device="cpu").transpose(0, 1), lay, i(2))
+
+
+def test_states_without_such_a_cache():
+    from types import SimpleNamespace
+
+    from lit_llama.state import SequenceState
+
+    model = SimpleNamespace(mixers=[SimpleNamespace(ring_window=lambda: 8), SimpleNamespace(ring_window=lambda: None)])
+    with pytest.raises(ValueError, match="4 bits"):
+        SequenceState(model, 1, None, "int4")
+    with pytest.raises(ValueError, match="int4"):
+        SequenceState(model, 1, None, "int8")
+
+
+def test_rows_of_an_item():
+    from lit_llama import kv4
+
+    lay = kv4.Layout(8, 128, 128, 64)
+    assert kv4.item_rows(lay, 32, 1, torch.bfloat16) == 4 and kv4.item_rows(lay, 32, 16, torch.bfloat16) == 4
+    assert kv4.item_rows(lay, 32, 17, torch.bfloat16) == 32 and kv4.item_rows(lay, 32, 17, torch.float32) == 16
+    assert kv4.item_rows(kv4.Layout(1, 200, 64, 16), 20, 500, torch.bfloat16) == 3 and kv4.item_rows(kv4.Layout(1, 64, 64, 16), 300, 1, torch.float32) == 1
