@@ -319,6 +319,71 @@ def test_what_stands_behind_a_row_is_not_read(hip, dtype, per):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_nan_behind_a_prompts_row(hip, dtype):
+    """The same among prompt rows, which share their tiles: NaN at position 90 reaches rows 90 .. 129 and no others."""
+    from lit_llama import kv4
+
+    c = Case([130], [130], 2, 1, 64, 64, 32, dtype)
+    at = int(c.table[c.slot[0].item(), 2]) * 32 + 90 - 64
+    nan = torch.full((1, 1, 64), float("nan"), dtype=dtype, device="cuda")
+    kv4.write(c.pool, c.lay, nan, nan, ints([at]))
+    y = c.run(64)
+    assert y[90:].isnan().all()
+    want, tol = c.want()
+    assert (np.abs(y.double().cpu().numpy() - want) <= tol)[:90].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pages_far_into_a_large_pool(hip, dtype):
+    """Places whose bytes lie past 2^32: rows written, read and attended to as at the pool's beginning."""
+    from lit_llama import kv4
+
+    lay = kv4.Layout(1, 128, 128, 64)
+    n = (1 << 32) // lay.block_bytes() + 40
+    pool = torch.empty(n, 1, lay.block_bytes(), dtype=torch.uint8, device="cuda")
+    g = np.random.default_rng(1)
+    L = 700
+    k, v = (rounded(x, dtype)[1] for x in (keys(g, L, 1, 128), g.standard_normal((L, 1, 128))))
+    q = rounded(g.standard_normal((40, 4 * 128)), dtype)[1]
+    out = []
+    for ids in (range(0, 11), range(n - 11, n)):
+        place = ints([ids[t // 64] * 64 + t % 64 for t in range(L)])
+        kv4.write(pool, lay, k, v, place)
+        a = kv4.read(pool, lay, place, dtype)
+        table = ints([list(ids)])
+        y = kv4.attend(q[:1], pool, lay, table, ints([0]), ints([L - 1]))
+        z = kv4.attend(q, pool, lay, table, ints([0]), ints(range(L - 40, L)), work=ints([[0, 40, 0]]), rows=40)
+        out.append((*a, y, z))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompt_rows_in_a_graph(hip, dtype):
+    """Rows behind a long cache, in key ranges that a second launch joins, captured and replayed over new queries and lengths."""
+    from lit_llama import kv4
+
+    c = Case([2600], [40], 8, 2, 64, 64, 64, dtype, seed=3)
+    work, pos, q = c.work(40), ints(c.pos), c.qd.clone()
+    assert kv4.splits(c.lay, 8, 1, 40, 2600, dtype)[0] > 1
+    kv4.attend(q, c.pool, c.lay, c.table, c.slot, pos, work=work, rows=40)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = kv4.attend(q, c.pool, c.lay, c.table, c.slot, pos, work=work, rows=40)
+    for turn in range(3):
+        first = [2559, 100, -3][turn]
+        c.pos = [first + i for i in range(40)]
+        c.q, qd = rounded(np.random.default_rng(turn).standard_normal(c.q.shape), dtype)
+        q.copy_(qd)
+        pos.copy_(ints(c.pos))
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(y)
+        assert torch.equal(y, kv4.attend(qd, c.pool, c.lay, c.table, c.slot, ints(c.pos), work=work, rows=40))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_strided_rows_and_outputs(hip, dtype):
     """Queries and gates out of packed projections at odd columns, into a wider output; rows of no item are left as they were."""
     c = Case([100, 41, 7], [1, 1, 1], 6, 2, 64, 64, 16, dtype, seed=2)

@@ -184,6 +184,14 @@ def test_steps_in_a_captured_graph(hip):
     assert int(t.fault) == 1 and int(r.status) == 1 and r.place.tolist() == [-1] * 3 and int(t.nfree) == 0
 
 
+def test_calls_without_rows(hip):
+    """Sequences that add nothing and no room for rows: lengths and first rows come back all the same."""
+    t = Both(3, 4, 9, 16)
+    t.check([2, 0], [5, 16])
+    r = t.check([0, 2, 1], [0, 0, 0], chunk=4)
+    assert r.seen.tolist() == [16, 5, 0] and r.pos.numel() == 0
+
+
 def test_on_another_stream(hip):
     t = Both(3, 8, 20, 16)
     s = torch.cuda.Stream()
