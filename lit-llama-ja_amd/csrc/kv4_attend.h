@@ -3,11 +3,15 @@
 // Codes enter the matrix products as exact small integers, made two at a time by one and-or (16 + c) and, where it costs little, one
 // subtraction more (c - 8); scales and offsets are applied in fp32, to the scores and to the weights, so nothing of a key or value is rounded:
 //   sum_j p s' c' = sum_j (p s') (c' + bias) - bias sum_j p s',  and sum_j p o':  two scalars a row.
-// Queries: bf16 rows as they are, fp32 rows as three bf16 terms (all 24 bits). Weights 2^6 p s' / m, m a power of two up to the largest s' so far, p
-// for a maximum that is raised once the scores pass it by kSlack octaves (raising it costs a pass over the accumulators, which the first tens of
-// tiles would otherwise all pay): below 2^15, and weights of 2^-20 of the largest are still normal numbers. fp16, whose 11 bits are 8 times
-// finer than the output's; fp32 rows two fp16 terms, 22 bits. Where the bias is 16 its scalar sums the rounded weights: the roundings then weigh |c' + bias| -
-// |bias|, not 3 times the values (0.0020 instead of 0.0017 off in the norm). fp32 rows take c - 8 throughout.
+// Queries: bf16 rows as they are, fp32 rows as three bf16 terms (all 24 bits).
+// p is taken for a reference that is raised, kv4_slack octaves past the maximum, once a score passes it: p <= 1, and the passes over the
+// accumulators that raising costs are few. Weights enter as 2^6 p s' / u with a power of two u of each column's own, up to its largest p s' when u
+// was set, and raised once a weight would pass 2^15: weights of 2^-20 of the column's largest are still normal numbers. (One u from the largest s' of
+// the tile lost a row its own values once a key of the tile that it does not see, or sees with p near 0, had 2^20 times their scale.) Both checks
+// are made on each lane's own keys; only where one fires are the lanes of a column put together.
+// fp16, whose 11 bits are 8 times finer than the output's; fp32 rows two fp16 terms, 22 bits. Where the bias is 16 its scalar sums the rounded
+// weights: the roundings then weigh |c' + bias| - |bias|, not 3 times the values (0.0020 instead of 0.0017 off in the norm). fp32 rows take c - 8
+// throughout.
 #pragma once
 #include "elem.h"
 #include "kv4.h"
@@ -133,12 +137,21 @@ __device__ __forceinline__ float groups_sum(float v) {
   return a + b;
 }
 
-// The weights' unit: the power of two up to the largest scale (at least kScaleMin; bf16 scales end far below 2^126), and 2^6 over it
-constexpr float kScaleMin = 7.8886e-31f;  // 2^-100
-constexpr float kSlack = 8.f;
+constexpr float kv4_slack(bool f32) { return f32 ? 2.f : 8.f; }  // (fp32 rows: differences of 8 octaves would cost a weight its last two bits)
+
+// A column's unit u: a power of two, at least kUnitMin (the largest bf16 scale is below 2^126), and 2^6 over it
+constexpr float kUnitMin = 7.5231638e-37f;  // 2^-120
+constexpr float kUnitPast = 512.f;          // raised by a weight past so many of it
 __device__ __forceinline__ float pow2_floor(float x) { return __uint_as_float(__float_as_uint(x) & 0x7F800000u); }
 __device__ __forceinline__ float weight_unit(float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)) * 64.f; }
 constexpr float kUnweight = 1.f / 64.f;
+// A new unit for what is held times corr and for weights up to top; corr becomes the factor of what is held
+__device__ __forceinline__ void kv4_raise(float top, float& unit, float& up, float& corr) {
+  const float kept = unit * corr;
+  unit = pow2_floor(fmaxf(fmaxf(kept, top), kUnitMin));
+  up = weight_unit(unit);
+  corr = kept * (up * kUnweight);
+}
 
 // One item's columns, (row, query head) pairs of one K / V head: column c is row c / R, head c % R
 struct Kv4Columns {

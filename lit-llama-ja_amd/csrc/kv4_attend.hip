@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
 
   u32x4 qf[NQ][KT];
   const float qs = kv4_query<T, KT, NQ>(p, row, head, g, qf), sl2 = kv4_scale(p), qi = F32 ? 0.f : -16.f * qs;
-  const float slack = kSlack / sl2;
+  const float slack = kv4_slack(F32) / sl2;
   const f32x4 begin = {qi, qi, qi, qi};
 
   // ---- a step's codes and pairs. Each is fetched anew right behind its use, for the wave's next step: no copies, and every load has most of a step
@@ -166,8 +166,8 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     }
   };
 
-  float m_run = -INFINITY, l_run = 0.f, z_run = 0.f, b_run = 0.f;  // maximum of column col; this lane's share of its sums of p, p o', weights
-  float unit = kScaleMin, up = weight_unit(unit);       // of the weights (uniform)
+  float m_run = -INFINITY, l_run = 0.f, z_run = 0.f, b_run = 0.f;  // column col's reference; this lane's share of its sums of p, p o', weights
+  float unit = kUnitMin, up = weight_unit(unit);                   // of its weights
   f32x4 acc[4 * VH];
 #pragma unroll
   for (int d = 0; d < 4 * VH; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -234,43 +234,47 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
           }
       }
     }
-    float mx = -INFINITY, ms = kScaleMin;
+    float mx = -INFINITY, corr = 1.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sm[j][i]);
+    const bool raise = __any(mx > m_run);
+    if (raise) {
+      mx = groups_max(over_banks<PACK>(mx, [](float a, float b) { return fmaxf(a, b); }));
+      const float m_new = mx > m_run ? mx + slack : m_run;
+      corr = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * sl2);
+      m_run = m_new;
+      l_run *= corr;
+      z_run *= corr;
+    }
+    const float mu = m_run == -INFINITY ? 0.f : m_run, mus = mu * sl2;
+    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mx = fmaxf(mx, sm[j][i]);
-        ms = fmaxf(ms, bflo(vp[j][i]));
+        const float e = kv4_weight<F32>(sm[j][i], mu, mus, sl2);
+        l_run += e;
+        z_run = fmaf(e, bfhi(vp[j][i]), z_run);
+        sm[j][i] = e * bflo(vp[j][i]);
+        top = fmaxf(top, sm[j][i]);
       }
-    mx = over_banks<PACK>(mx, [](float a, float b) { return fmaxf(a, b); });
-    mx = groups_max(mx);
-    ms = groups_max(masked || PACK > 1 ? row16_max(ms) : ms);
-    if (__any(mx > m_run + slack) || ms > unit + unit) {  // (uniform) a new maximum, or larger scales
-      const float m_new = fmaxf(m_run, mx), grown = fmaxf(unit, pow2_floor(ms));
-      float corr = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * sl2);
-      m_run = m_new;
-      l_run *= corr;
-      z_run *= corr;
-      corr *= unit / grown;
+    if (raise || __any(top > kUnitPast * unit)) {
+      kv4_raise(groups_max(over_banks<PACK>(top, [](float a, float b) { return fmaxf(a, b); })), unit, up, corr);
       b_run *= corr;
-      unit = grown;
-      up = weight_unit(unit);
 #pragma unroll
       for (int d = 0; d < 4 * VH; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[d][i] *= corr;
     }
-    const float mu = m_run == -INFINITY ? 0.f : m_run, mus = mu * sl2;
     uint32_t pm[NJ][2][NP], pt[NB][2][NP];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = kv4_weight<F32>(sm[j][i], mu, mus, sl2);
-        l_run += e;
-        z_run = fmaf(e, bfhi(vp[j][i]), z_run);
-        w[i] = e * (bflo(vp[j][i]) * up);
+        w[i] = sm[j][i] * up;
         if (F32) b_run += w[i];
       }
       split_h<NP>(w[0], w[1], pm[j][0]);

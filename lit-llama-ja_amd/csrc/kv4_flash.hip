@@ -16,7 +16,7 @@ namespace llj {
 template <int KT, int VH>
 struct Kv4Tile {
   static constexpr int kKeys = 4 * KT * 1024, kValues = 8 * VH * 1024;  // bytes of unpacked keys, values
-  static constexpr int kPairs = kKeys + kValues, kTop = kPairs + 1024, kBytes = kTop + 32;  // (pairs: key scales, offsets, value scales, offsets)
+  static constexpr int kPairs = kKeys + kValues, kHere = kPairs + 1024, kBytes = kHere + 16;  // (pairs: key scales, offsets, value scales, offsets; here: 16 keys' page exists)
 };
 
 template <typename T, int KT, int VH, int QB>
@@ -43,7 +43,8 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   if (cols.n <= 0) return;
   const int sl = p.slot[b];
   const bool held = sl >= 0 && sl < p.slots;
-  const int* tab = p.table + (size_t)(held ? sl : 0) * p.ldt + vzero();  // (loaded into vector registers, moved to scalar ones a tile later: a move at the load would wait for it)
+  // (page numbers are loaded into vector registers and moved to scalar ones a tile later: a move at the load would wait for it)
+  const int* tab = p.table + (size_t)(held ? sl : 0) * p.ldt + vzero();
   const int k = p.pool.k, pmask = (1 << k) - 1, most = held ? (p.ldt << k) - 1 : -1;
   // the last position any column sees (a lane a column)
   int plast = -1;
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   int row[QB], head[QB], pc[QB], wfirst = 0x7fffffff;
   u32x4 qf[QB][NQ][KT];
   float qs[QB], qi[QB];
-  const float sl2 = kv4_scale(p), slack = kSlack / sl2;
+  const float sl2 = kv4_scale(p), slack = kv4_slack(F32) / sl2;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     const int c = (wave * QB + q) * 16 + col;
@@ -143,16 +144,17 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
     float* at = reinterpret_cast<float*>(buf + Tile::kPairs + (lane & 16) * 32) + wave * 16 + col;  // (lanes 32 .. 63 write the same)
     at[0] = sc;
     at[64] = of;
-    const float top = row16_max(sc);  // of the values' scales in the odd rows of lanes; -1: keys that are not there. (The keys' go behind)
-    *reinterpret_cast<float*>(buf + Tile::kTop + 16 - (lane & 16) + 4 * wave) = ok ? top : -1.f;
+    if (lane == 0) *reinterpret_cast<float*>(buf + Tile::kHere + 4 * wave) = ok ? 1.f : -1.f;
   };
 
-  float m_run[QB], l_run[QB], z_run[QB], unit = kScaleMin, up = weight_unit(unit);
+  float m_run[QB], l_run[QB], z_run[QB], unit[QB], up[QB];
   f32x4 acc[QB][4 * VH];
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     m_run[q] = -INFINITY;
     l_run[q] = z_run[q] = 0.f;
+    unit[q] = kUnitMin;
+    up[q] = weight_unit(kUnitMin);
 #pragma unroll
     for (int d = 0; d < 4 * VH; ++d) acc[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -170,153 +172,151 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
   for (int t = t0; t < t1; ++t) {
     const uint8_t* buf = lds + ((t - t0) & 1) * Tile::kBytes;
     uint8_t* then = lds + ((t + 1 - t0) & 1) * Tile::kBytes;  // (its last readers passed the barrier before this tile)
-    {
-      f32x4 s[QB][4];
+    f32x4 s[QB][4];
 #pragma unroll
-      for (int q = 0; q < QB; ++q)
+    for (int q = 0; q < QB; ++q)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[q][j] = f32x4{qi[q], qi[q], qi[q], qi[q]};
-      // Operands are read ahead of their products, fences keep the compiler from reading each right before its use (which left the LDS latency
-      // open 30 times a tile)
-      u32x4 a[2][8];
-      f32x4 sc[4], of[4];
-      const f32x4* pairs = reinterpret_cast<const f32x4*>(buf + Tile::kPairs) + g;
-      auto keys = [&](int c) {
+      for (int j = 0; j < 4; ++j) s[q][j] = f32x4{qi[q], qi[q], qi[q], qi[q]};
+    // Operands are read ahead of their products, fences keep the compiler from reading each right before its use (which left the LDS latency
+    // open 30 times a tile)
+    u32x4 a[2][8];
+    f32x4 sc[4], of[4];
+    const f32x4* pairs = reinterpret_cast<const f32x4*>(buf + Tile::kPairs) + g;
+    auto keys = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[c & 1][i] = *reinterpret_cast<const u32x4*>(buf + (8 * c + i) * 1024 + lane * 16);
-      };
-      auto products = [&](int c) {
+      for (int i = 0; i < 8; ++i) a[c & 1][i] = *reinterpret_cast<const u32x4*>(buf + (8 * c + i) * 1024 + lane * 16);
+    };
+    auto products = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int q = 0; q < QB; ++q)
-#pragma unroll
-            for (int e = 0; e < NQ; ++e)
-              s[q][i & 3] = mfma_bf16(__builtin_bit_cast(bf16x8, a[c & 1][i]), __builtin_bit_cast(bf16x8, qf[q][e][2 * c + (i >> 2)]), s[q][i & 3]);
-      };
-      keys(0);
-#pragma unroll
-      for (int c = 0; c < KT / 2; ++c) {
-        if (c + 1 < KT / 2) keys(c + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        if (c == 0) unpack(then);
-        products(c);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sc[j] = pairs[4 * j];
-        of[j] = pairs[16 + 4 * j];
-      }
-      fetch(last(t + 2), uniform(next));
-      next = page_of(last(t + 3));
-      const f32x4 tops = *reinterpret_cast<const f32x4*>(buf + Tile::kTop);
-      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      const bool gap = uniform(fminf(fminf(tops[0], tops[1]), fminf(tops[2], tops[3])) < 0.f);
-      const bool masked = gap || 64 * t + 63 > wfirst;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int q = 0; q < QB; ++q) s[q][j] = kv4_scores(s[q][j], sc[j], of[j], qs[q]);
-      if (masked) {
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int q = 0; q < QB; ++q)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int lim = tops[j] < 0.f ? -1 : pc[q];
+          for (int e = 0; e < NQ; ++e)
+            s[q][i & 3] = mfma_bf16(__builtin_bit_cast(bf16x8, a[c & 1][i]), __builtin_bit_cast(bf16x8, qf[q][e][2 * c + (i >> 2)]), s[q][i & 3]);
+    };
+    keys(0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (64 * t + 16 * j + 4 * g + i > lim) s[q][j][i] = -INFINITY;
-          }
-      }
-      float mx[QB];
-      bool raise = top > unit + unit;
+    for (int c = 0; c < KT / 2; ++c) {
+      if (c + 1 < KT / 2) keys(c + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (c == 0) unpack(then);
+      products(c);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        mx[q] = -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      sc[j] = pairs[4 * j];
+      of[j] = pairs[16 + 4 * j];
+    }
+    fetch(last(t + 2), uniform(next));
+    next = page_of(last(t + 3));
+    const f32x4 here = *reinterpret_cast<const f32x4*>(buf + Tile::kHere);
+    const bool gap = uniform(fminf(fminf(here[0], here[1]), fminf(here[2], here[3])) < 0.f);
+    const bool masked = gap || 64 * t + 63 > wfirst;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[q] = fmaxf(mx[q], s[q][j][i]);
-        mx[q] = groups_max(mx[q]);
-        raise |= mx[q] > m_run[q] + slack;
-      }
-      if (__any(raise)) {  // a new maximum, or larger scales
-        const float grown = fmaxf(unit, pow2_floor(top));
+      for (int q = 0; q < QB; ++q) s[q][j] = kv4_scores(s[q][j], sc[j], of[j], qs[q]);
+    if (masked) {
 #pragma unroll
-        for (int q = 0; q < QB; ++q) {
-          const float m_new = fmaxf(m_run[q], mx[q]);
-          float corr = m_run[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[q] - m_new) * sl2);
-          m_run[q] = m_new;
-          l_run[q] *= corr;
-          z_run[q] *= corr;
-          corr *= unit / grown;
-#pragma unroll
-          for (int d = 0; d < 4 * VH; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[q][d][i] *= corr;
-        }
-        unit = grown;
-        up = weight_unit(unit);
-      }
-      u32x4 va[2][4 * VH];
-      f32x4 sv[4], zv[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sv[j] = pairs[32 + 4 * j] * up;
-        zv[j] = pairs[48 + 4 * j];
-      }
-      auto weights = [&](int q, auto some, uint32_t (&pt)[4][2][NP]) {  // (some: keys that a column does not see, whose values may be NaN)
-        const float mu = m_run[q] == -INFINITY ? 0.f : m_run[q], mus = mu * sl2;
+      for (int q = 0; q < QB; ++q)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float w[4];
+          const int lim = here[j] < 0.f ? -1 : pc[q];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = kv4_weight<F32>(s[q][j][i], mu, mus, sl2);
-            const bool seen = !some || s[q][j][i] != -INFINITY;
-            l_run[q] += e;
-            z_run[q] = fmaf(e, seen ? zv[j][i] : 0.f, z_run[q]);
-            w[i] = e * (seen ? sv[j][i] : 0.f);
-          }
-          split_h<NP>(w[0], w[1], pt[j][0]);
-          split_h<NP>(w[2], w[3], pt[j][1]);
+          for (int i = 0; i < 4; ++i)
+            if (64 * t + 16 * j + 4 * g + i > lim) s[q][j][i] = -INFINITY;
         }
-      };
-      auto values = [&](int u) {
+    }
+    float mx[QB], corr[QB], top[QB];
+    bool raise = false;
 #pragma unroll
-        for (int d = 0; d < 4 * VH; ++d) va[u][d] = *reinterpret_cast<const u32x4*>(buf + Tile::kKeys + (u * 4 * VH + d) * 1024 + lane * 16);
-      };
-      auto add = [&](int q, int u, const uint32_t (&pt)[4][2][NP]) {
+    for (int q = 0; q < QB; ++q) {
+      mx[q] = -INFINITY;
+      corr[q] = 1.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[q] = fmaxf(mx[q], s[q][j][i]);
+      raise |= mx[q] > m_run[q];
+    }
+    raise = __any(raise);
+    if (raise) {
+#pragma unroll
+      for (int q = 0; q < QB; ++q) {
+        mx[q] = groups_max(mx[q]);
+        const float m_new = mx[q] > m_run[q] ? mx[q] + slack : m_run[q];
+        corr[q] = m_run[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[q] - m_new) * sl2);
+        m_run[q] = m_new;
+        l_run[q] *= corr[q];
+        z_run[q] *= corr[q];
+      }
+    }
+    u32x4 va[2][4 * VH];
+    f32x4 sv[4], zv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sv[j] = pairs[32 + 4 * j];
+      zv[j] = pairs[48 + 4 * j];
+    }
+    auto weights = [&](int q, auto some) {  // (some: keys that a column does not see, whose values may be NaN)
+      const float mu = m_run[q] == -INFINITY ? 0.f : m_run[q], mus = mu * sl2;
+      top[q] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = kv4_weight<F32>(s[q][j][i], mu, mus, sl2);
+          const bool seen = !some || s[q][j][i] != -INFINITY;
+          l_run[q] += e;
+          z_run[q] = fmaf(e, seen ? zv[j][i] : 0.f, z_run[q]);
+          s[q][j][i] = e * (seen ? sv[j][i] : 0.f);
+          top[q] = fmaxf(top[q], s[q][j][i]);
+        }
+    };
+    auto values = [&](int u) {
+#pragma unroll
+      for (int d = 0; d < 4 * VH; ++d) va[u][d] = *reinterpret_cast<const u32x4*>(buf + Tile::kKeys + (u * 4 * VH + d) * 1024 + lane * 16);
+    };
+    auto add = [&](int q, int u, const uint32_t (&pt)[4][2][NP]) {
+#pragma unroll
+      for (int d = 0; d < 4 * VH; ++d)
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          acc[q][d] = mfma_f16(va[u][d], u32x4{pt[2 * u][0][i], pt[2 * u][1][i], pt[2 * u + 1][0][i], pt[2 * u + 1][1][i]}, acc[q][d]);
+    };
+    uint32_t pt[QB][4][2][NP];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+      if (masked) weights(q, std::true_type{});
+      else weights(q, std::false_type{});
+      if (raise || __any(top[q] > kUnitPast * unit[q])) {
+        kv4_raise(groups_max(top[q]), unit[q], up[q], corr[q]);
 #pragma unroll
         for (int d = 0; d < 4 * VH; ++d)
 #pragma unroll
-          for (int i = 0; i < NP; ++i)
-            acc[q][d] = mfma_f16(va[u][d], u32x4{pt[2 * u][0][i], pt[2 * u][1][i], pt[2 * u + 1][0][i], pt[2 * u + 1][1][i]}, acc[q][d]);
-      };
-      uint32_t pt[QB][4][2][NP];
-      if (masked) {
-#pragma unroll
-        for (int q = 0; q < QB; ++q) weights(q, std::true_type{}, pt[q]);
-      } else {
-#pragma unroll
-        for (int q = 0; q < QB; ++q) weights(q, std::false_type{}, pt[q]);
+          for (int i = 0; i < 4; ++i) acc[q][d][i] *= corr[q];
       }
-      values(0);  // (the scores' registers are free now)
-      values(1);
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int q = 0; q < QB; ++q) add(q, u, pt[q]);
+      for (int j = 0; j < 4; ++j) {
+        split_h<NP>(s[q][j][0] * up[q], s[q][j][1] * up[q], pt[q][j][0]);
+        split_h<NP>(s[q][j][2] * up[q], s[q][j][3] * up[q], pt[q][j][1]);
+      }
     }
+    values(0);  // (the scores' registers are free now)
+    values(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int q = 0; q < QB; ++q) add(q, u, pt[q]);
     __syncthreads();
   }
   // ---- lane (col, g) holds values VW / 4 g + 4 VH i + 4 v + d of its columns
-  const float down = unit * kUnweight;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    const float l = groups_sum(l_run[q]), z = groups_sum(z_run[q]), m = m_run[q] * sl2;
+    const float down = unit[q] * kUnweight, l = groups_sum(l_run[q]), z = groups_sum(z_run[q]), m = m_run[q] * sl2;
     if ((wave * QB + q) * 16 + col < cols.n) {
       const float f = p.nsplit == 1 ? kv4_factor<T>(p, row[q], head[q], m, l) : 1.f;
       float* dst = p.nsplit == 1 ? nullptr : kv4_part<VW>(p, row[q], head[q], sp);

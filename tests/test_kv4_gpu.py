@@ -6,9 +6,9 @@ Codes, scales and offsets are compared bit for bit. Attention's tolerance, for r
     |error| <= e = (D + 8) 2^-24 scale (31 s + |o|) sum |q| at most, the queries themselves exact (three bf16 terms);
     every weight is then off by a factor exp(2 e) at most (its own score and the sum's), and by 2^-21 from exp2, whose argument is rounded: 2^-23
     |score - top|, both times max |v|;
-  * a weight times its scale enters as one fp16 number (2^-12, below the 2^-16 allowed here times 31 s instead of 7.5 s only in the mean: a bf16
-    output's own 2^-8 covers it) or as two (22 bits, 2^-23; allowed: 2^-24 of four times the values) and is summed over n keys in fp32, n 2^-24,
-    beside 16 + c: times (31 s + |o|) of the values.
+  * a weight times its scale enters as one fp16 number or as two, and is summed over n keys in fp32, n 2^-24, beside 16 + c: times (31 s + |o|) of
+    the values. Of two numbers (22 bits) 2^-24 is allowed. Of one, off by 2^-12 p (15 s) in one term, the sum is off by less than the bf16 output's
+    own 2^-9 (counted as 2^-8 |y|) wherever |y| is of the values' size; 2^-16 is allowed beside it where it is not.
 """
 import numpy as np
 import pytest
@@ -331,6 +331,66 @@ def test_nan_behind_a_prompts_row(hip, dtype):
     assert y[90:].isnan().all()
     want, tol = c.want()
     assert (np.abs(y.double().cpu().numpy() - want) <= tol)[:90].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_tile_of_nan_behind_a_prompts_row(hip, dtype):
+    """Positions 64 .. 127 all NaN, a tile of keys without one scale: rows 0 .. 63 of the same item do not see them."""
+    from lit_llama import kv4
+
+    c = Case([130], [130], 2, 1, 64, 64, 64, dtype)
+    at = int(c.table[c.slot[0].item(), 1]) * 64
+    nan = torch.full((64, 1, 64), float("nan"), dtype=dtype, device="cuda")
+    kv4.write(c.pool, c.lay, nan, nan, ints(range(at, at + 64)))
+    y = c.run(64)
+    assert y[64:].isnan().all()
+    want, tol = c.want()
+    assert (np.abs(y.double().cpu().numpy() - want) <= tol)[:64].all()
+
+
+def put(c, b, places, k=None, v=None):
+    """Keys, values (t, G, n) of sequence b at these places replaced, in the cache and in what is expected."""
+    from lit_llama import kv4
+
+    row = c.table[c.slot[b].item()].tolist()
+    k = rounded(c.k[b][places] if k is None else k, torch.float32)
+    v = rounded(c.v[b][places] if v is None else v, torch.float32)
+    kv4.write(c.pool, c.lay, k[1], v[1], ints([row[t // c.page] * c.page + t % c.page for t in places]))
+    c.k[b][places], c.v[b][places] = O.stands_for(k[0]), O.stands_for(v[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [64, 128])
+@pytest.mark.parametrize("rows,per", [(6, 8), (130, 64)])
+def test_large_values_behind_a_row(hip, dtype, n, rows, per):
+    """A value 2^30 times the others: rows before its position keep every digit of theirs, in one item with the rows that see it."""
+    c = Case([150], [rows], 2, 1, n, n, 32, dtype, seed=n)
+    put(c, 0, [146], v=c.g.standard_normal((1, 1, n)) * 2.0 ** 30)
+    c.check(c.run(per))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("low", [[300], list(range(128)), list(range(3, 690, 7))])
+@pytest.mark.parametrize("rows,per", [(1, None), (4, 8), (130, 64)])
+def test_large_values_of_keys_that_do_not_count(hip, dtype, low, rows, per):
+    """Seen keys whose scores are 60 and more below the others', e^-60 of their weights, with values 2^30 times the others': less than 2^-56 of a
+    result, so it is expected as if they were not there (and the others' weights, relative to the largest value and score among them, as precise)."""
+    c = Case([820], [rows], 2, 1, 64, 64, 64, dtype, seed=4)
+    q = c.q.reshape(rows, 2, 64)
+    q[:, :, 0] = 20
+    c.q, c.qd = rounded(q.reshape(rows, -1), dtype)
+    every = np.arange(820)
+    put(c, 0, every, k=np.where(np.arange(64) == 0, np.clip(c.k[0], -2, 2), c.k[0]))
+    put(c, 0, low, k=np.broadcast_to(np.where(np.arange(64) == 0, -40.0, 0.0), (len(low), 1, 64)),
+        v=c.g.standard_normal((len(low), 1, 64)) * 2.0 ** 30)
+    y = c.run(per)
+    s = np.einsum("mhd,td->mht", c.q.reshape(rows, 2, 64), c.k[0][:, 0]) / 8
+    keep = np.setdiff1d(every, low)
+    first = 820 - rows
+    assert (s[:, :, keep[keep <= first]].max(2) - s[:, :, low].max(2) > 60).all()
+    c.k[0], c.v[0] = c.k[0][keep], c.v[0][keep]
+    c.pos = [p - len(low) for p in c.pos]
+    c.check(y)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
