@@ -669,7 +669,7 @@ int llj_pages_release(const int* slot, int B, int* seen, int slots, int* table, 
  * largest bf16 up to the smallest value, s = (largest - o) / 15 rounded to fp32, then bf16, c = (x - o) / s rounded to the nearest
  * (halves to even) and kept in 0 .. 15, all 0 where s is. A vector with an infinity or NaN, or a value below bf16's range, is NaN.
  * write: row m's keys k[m ldk + head hk + i] and values into place[m] (outside the pool: the row is left out; the places of a call differ).
- * read: what stands there, in bf16 or fp32 (outside: zeros). */
+ * read: what stands there, in bf16 or fp32 (outside: zeros). M kv_heads up to 2^26 a call. */
 size_t llj_kv4_block_bytes(int page, int dim, int vdim);
 int llj_kv4_write(const void* k, size_t ldk, size_t hk, const void* v, size_t ldv, size_t hv, const int* place, int M, int kv_heads, int dim,
                   int vdim, int dt, void* pool, int pages, int page, void* stream);

@@ -184,7 +184,7 @@ template <bool WRITE>
 static int kv4_io(void* pool, int pages, int page, int G, void* k, size_t ldk, size_t hk, void* v, size_t ldv, size_t hv, const int* place,
                   int M, int D, int V, int dt, void* stream) {
   LLJ_REQUIRE(kv4_sizes(pool, pages, page, G, D, V, dt) && k && v && place && M >= 0 && ((ldk | hk | ldv | hv) >> 40) == 0 &&
-              (long long)M * G <= 1LL << 31);
+              (long long)M * G <= 1 << 26);  // (a grid's threads stay below 2^32)
   if (M == 0) return 0;
   Kv4IO io{};
   io.pool = kv4_pool(pool, pages, G, kv4_page_log2(page), D, V);

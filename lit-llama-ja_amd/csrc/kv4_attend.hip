@@ -422,7 +422,7 @@ int llj_kv4_attend(const void* q, int ldq, const void* gate, int ldg, const int*
               ((uintptr_t)part & 15) == 0 && ((uintptr_t)count & 3) == 0 && (work || (rows == 1 && items <= M && items <= B)));
   const int tiles = llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt);
   const bool few = rows * (heads / kv_heads) <= kv4_few_columns;
-  LLJ_REQUIRE(tiles > 0 && (long long)items * tiles <= 0x7fffffff && (nsplit == 1 || !few || count));
+  LLJ_REQUIRE(tiles > 0 && (long long)items * tiles < 1 << 24 && (nsplit == 1 || !few || count));
   if (items == 0 || M == 0) return 0;
   Kv4Attend p{};
   p.q = q; p.gate = gate; p.ldq = ldq; p.ldg = ldg; p.work = work; p.items = items; p.rows = rows;

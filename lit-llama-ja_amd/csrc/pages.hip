@@ -20,6 +20,7 @@ constexpr int kMaxSeqs = 4096;    // three sums of 16 KiB in LDS
 constexpr int kMaxSlots = 65536;  // a bit each in LDS
 constexpr int kPlanThreads = 1024;
 constexpr int kSat = 0x3fffffff;  // sums saturate here: past every size that is taken
+constexpr int kMaxTokens = 1 << 30;  // of a sequence
 constexpr int kFewRows = 4096;    // calls up to this many rows and items are one launch
 
 struct ExtendParams {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
         const int L = p.seen[s];
         // (L + n at most 2^31 - 1 in unsigned arithmetic, then against the table's width)
         const unsigned need = (((unsigned)L + (unsigned)n) + page - 1) >> p.k;
-        if (L < 0 || L > kSat || need > (unsigned)p.ldt) ok = false;
+        if (L < 0 || L > kMaxTokens || need > (unsigned)p.ldt) ok = false;
         if (ok) {
           v[0] = n;
           v[1] = (int)need - ((L + page - 1) >> p.k);
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_release_kernel(ReleasePara
         const unsigned bit = 1u << (s & 31);
         if (atomicOr(&s_used[s >> 5], bit) & bit) ok = false;
         const int L = p.seen[s];
-        if (L < 0 || L > kSat || ((L + page - 1) >> p.k) > p.ldt) ok = false;
+        if (L < 0 || L > kMaxTokens || ((L + page - 1) >> p.k) > p.ldt) ok = false;
         else v[0] = (L + page - 1) >> p.k;
       }
       if (!ok) atomicOr(&s_bad, 2);

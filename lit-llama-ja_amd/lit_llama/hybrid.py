@@ -125,6 +125,7 @@ class HybridModel(torch.nn.Module):
         state.room(slots, [s + len(t) for s, t in zip(starts, tokens)])
         logits = torch.empty(n, self.head.Np, dtype=self.dtype, device=self.device)
         self.run(rows, self.new_work(rows.M), state, logits, pick, _hip.stream(), taps)
+        state.check()
         return logits[:, :self.config.vocab_size]
 
     @torch.no_grad()

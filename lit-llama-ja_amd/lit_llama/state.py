@@ -103,9 +103,13 @@ class SequenceState:
         return moved
 
     def extend(self, rows: "Rows") -> pages.PageRows:
-        """Places in the pages for a call's rows (one block table for all layers), once a call."""
+        """Places in the pages for a call's rows (one block table for all layers), once a call. The rows go on where their sequences
+        end; a prompt-style call at other positions is a fault (`check`)."""
         add = None if rows.decode else rows.new_tokens()
-        return pages.extend(self.table, self.seen, self.free, self.nfree, rows.slot, add, rows.M, PAGE, fault=self.fault)
+        out = pages.extend(self.table, self.seen, self.free, self.nfree, rows.slot, add, rows.M, PAGE, fault=self.fault)
+        if not rows.decode:
+            self.fault.bitwise_or_((out.pos != rows.pos).any().int() << 2)
+        return out
 
     def ensure(self, length: int) -> bool:
         """Room for sequences of `length` tokens in the layers that keep every token; True if they moved (a captured
@@ -159,9 +163,9 @@ class SequenceState:
         return sum(t.numel() * t.element_size() for t in [*self.recurrent.values(), *self.ring.values(), *self.pool.values(), *own, self.prev])
 
     def check(self) -> None:
-        """Waits for the calls so far and raises if one of them found no place for its rows."""
+        """Waits for the calls so far and raises if one of them found no place for its rows, or had them elsewhere."""
         if self.cache is not None and int(self.fault):
-            raise RuntimeError("a call's rows found no pages: this state's sequences are not valid")
+            raise RuntimeError("a call's rows found no pages, or did not begin where their sequences end: this state's sequences are not valid")
 
 
 class Rows:

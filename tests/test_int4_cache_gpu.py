@@ -133,6 +133,17 @@ def test_generate_and_memory(hip):
     assert sum(p.numel() for p in four.pool.values()) < 0.3 * sum(2 * r.numel() for r in full.ring.values())
 
 
+def test_rows_that_begin_elsewhere(hip):
+    """A call goes on where its sequences end: one that begins before or behind that, or names a slot twice, raises."""
+    cfg, w, m = case("tiled", torch.bfloat16)
+    for starts, again in (([3], [0]), ([9], [0]), ([5, 5], [0, 0])):
+        st = m.new_state(2, cache="int4")
+        slot = st.alloc(1)
+        m.extend(st, slot, [0], [[1, 2, 3, 4, 5]])
+        with pytest.raises(RuntimeError, match="not valid"):
+            m.extend(st, [slot[k] for k in again], starts, [[1, 2]] * len(starts))
+
+
 def test_what_is_refused(hip):
     from lit_llama import LLaMA, LLaMAConfig
     import generate as G

@@ -7,8 +7,8 @@ Codes, scales and offsets are compared bit for bit. Attention's tolerance, for r
     every weight is then off by a factor exp(2 e) at most (its own score and the sum's), and by 2^-21 from exp2, whose argument is rounded: 2^-23
     |score - top|, both times max |v|;
   * a weight times its scale enters as one fp16 number or as two, and is summed over n keys in fp32, n 2^-24, beside 16 + c: times (31 s + |o|) of
-    the values. Of two numbers (22 bits) 2^-24 is allowed. Of one, off by 2^-12 p (15 s) in one term, the sum is off by less than the bf16 output's
-    own 2^-9 (counted as 2^-8 |y|) wherever |y| is of the values' size; 2^-16 is allowed beside it where it is not.
+    the values. Of two numbers (22 bits) 2^-24 is allowed. Of one, each off by up to 2^-11 p (15 s) and
+    of either sign, the bf16 output's own 2^-8 |y| covers it where |y| is of the values' size; 2^-16 is allowed beside it where it is not.
 """
 import numpy as np
 import pytest

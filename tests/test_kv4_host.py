@@ -100,7 +100,7 @@ def test_pages_refuse():
 def test_rows_refuse():
     good = dict(k=P, ldk=64, hk=32, v=P, ldv=64, hv=32, place=P, M=3, G=2, D=32, V=32, dt=0, pool=P, pages=4, page=16, stream=None)
     bad = [dict(k=None), dict(v=None), dict(place=None), dict(M=-1), dict(G=0), dict(G=5000), dict(D=0), dict(D=257), dict(V=0), dict(V=300), dict(dt=2),
-           dict(pool=None), dict(pool=P + 8), dict(pages=0), dict(pages=1 << 27), dict(page=20), dict(ldk=1 << 41), dict(hv=1 << 62)]
+           dict(pool=None), dict(pool=P + 8), dict(pages=0), dict(pages=1 << 27), dict(page=20), dict(ldk=1 << 41), dict(hv=1 << 62), dict(M=(1 << 25) + 1)]
     for b in bad:
         a = {**good, **b}
         assert lib().llj_kv4_write(*a.values()) == EINVAL, b
@@ -115,7 +115,8 @@ def test_attention_refuses():
            dict(table=None), dict(slots=0), dict(ldt=0), dict(ldt=1 << 27), dict(pool=None), dict(pool=P + 4), dict(pages=0), dict(page=30), dict(part=None),
            dict(count=None), dict(part=P + 4), dict(nsplit=0), dict(nsplit=65), dict(y=None), dict(ldy=255), dict(M=-1), dict(heads=0), dict(heads=3),
            dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(vdim=0), dict(vdim=260), dict(dt=2), dict(work=None), dict(work=None, rows=1, items=5, M=5),
-           dict(work=None, rows=1, items=3, M=2, B=4), dict(heads=70000, kv_heads=35000, ldq=1 << 30)]
+           dict(work=None, rows=1, items=3, M=2, B=4), dict(heads=70000, kv_heads=35000, ldq=1 << 30),
+           dict(items=1 << 23)]
     for b in bad:
         assert lib().llj_kv4_attend(*{**good, **b}.values()) == EINVAL, b
     assert lib().llj_kv4_attend(*{**good, "items": 0}.values()) == 0

@@ -100,6 +100,23 @@ def test_the_largest_tables(hip):
     t.check(slots[1:], [1] * 4)
 
 
+def test_a_sequence_of_2_to_the_30_tokens(hip):
+    """The longest there is: it stays in a call that adds nothing, takes no token more, and gives its pages back."""
+    from lit_llama import pages
+
+    width = 1 << 26
+    table = torch.arange(width, dtype=torch.int32, device="cuda").view(1, width)
+    seen, free, nfree, fault = ints([1 << 30]), torch.full((width,), -5, dtype=torch.int32, device="cuda"), ints([0]), ints([0])
+    args = table, seen, free, nfree
+    r = pages.extend(*args, ints([0]), ints([0]), 3, 16, fault=fault)
+    assert int(r.status) == 0 and r.seen.tolist() == [1 << 30] and r.pos.tolist() == [-1] * 3
+    r = pages.extend(*args, ints([0]), ints([1]), 3, 16)
+    assert int(r.status) == pages.BAD_CALL and r.pos.tolist() == [-1] * 3 and seen.tolist() == [1 << 30]
+    assert int(pages.release(*args, ints([0]), 16, fault=fault)) == 0 and fault.tolist() == [0]
+    assert nfree.tolist() == [width] and seen.tolist() == [0]
+    assert torch.equal(free, torch.arange(width, dtype=torch.int32, device="cuda")) and bool((table == -1).all())
+
+
 def test_without_commit_the_same_call_again(hip):
     t = Both(4, 10, 30, 16)
     t.check([1, 2], [20, 5])
