@@ -223,6 +223,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_attend_ke
     fetch_pairs(kp, p.pool.ks);
     const bool masked = gap || STEP * t + STEP - 1 > pfirst;  // (uniform)
     if (masked) {
+      asm volatile("");  // (else the compiler masks every step, by selections without a branch)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int lim = pick([&](int b) { return ok[b] ? pc : -1; }, j);

@@ -219,6 +219,7 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
 #pragma unroll
       for (int q = 0; q < QB; ++q) s[q][j] = kv4_scores(s[q][j], sc[j], of[j], qs[q]);
     if (masked) {
+      asm volatile("");  // (else the compiler masks every tile, by selections without a branch)
 #pragma unroll
       for (int q = 0; q < QB; ++q)
 #pragma unroll
