@@ -7,6 +7,7 @@ include/lit_llama_amd.h), so a token costs 0.27 of its bf16 bytes at heads of 12
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -24,6 +25,17 @@ RANGE, RANGES, RANGE_LONG = 256, 16, 1024
 FEW_COLUMNS = 64  # (row, head) pairs of a K / V head in an item: from more on it is prompt rows (csrc/kv4_attend.hip)
 
 
+# (sizes, functions of a few integers: asked of the library once each, a call into it takes five times as long)
+@lru_cache(None)
+def _block_bytes(page: int, dim: int, vdim: int) -> int:
+    return int(_hip.lib().llj_kv4_block_bytes(page, dim, vdim))
+
+
+@lru_cache(4096)
+def _tiles(heads: int, kv_heads: int, dim: int, vdim: int, rows: int, dt: int) -> int:
+    return int(_hip.lib().llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt))
+
+
 def _dt(t: torch.dtype) -> int:
     if t not in (torch.bfloat16, torch.float32):
         raise TypeError(f"rows are bfloat16 or float32, not {t}")
@@ -39,7 +51,7 @@ class Layout:
 
     def block_bytes(self) -> int:
         """Bytes of one head's part of a page."""
-        n = int(_hip.lib().llj_kv4_block_bytes(self.page, self.dim, self.vdim))
+        n = _block_bytes(self.page, self.dim, self.vdim)
         if n == 0 or self.kv_heads < 1:
             raise ValueError(f"{self}: pages of {PAGE_SIZES} tokens, heads of 1 to 256")
         return n
@@ -122,7 +134,7 @@ def read(pool: torch.Tensor, layout: Layout, place: torch.Tensor, dtype: torch.d
 
 def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: torch.dtype = torch.bfloat16) -> Tuple[int, int]:
     """(key ranges, counters) of a call of `items` items of up to `rows` rows over up to `keys` keys (prompt rows need no counters)."""
-    tiles = _hip.lib().llj_kv4_tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
+    tiles = _tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
     if not tiles:
         raise ValueError(f"{heads} heads on {layout.kv_heads}, items of {rows} rows")
     wgs, long = max(1, items * tiles), -(-keys // RANGE_LONG)
