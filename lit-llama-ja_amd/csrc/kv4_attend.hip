@@ -1,12 +1,17 @@
 // Attention of few rows per sequence over the paged 4-bit cache, split over the keys (mathematics: kv4_attend.h).
 //
 // One workgroup per (item, 16 columns of a K / V head, key range); a column is a (row, query head) pair, so heads that share a K / V head
-// and the rows of a short item share its bytes. Waves walk 16 NB keys at a time on their own (no barriers). K fragment: lane (r, g) holds words KT g .. KT g + KT - 1 of key r, one load of 4 KT bytes, and the
-// queries are loaded in that order. V fragment: lane (r, g) takes 4 VH columns of 8 keys; two keys' halves are permuted into one word first,
-// so no transposition is needed. A wave's results, then the workgroups', are merged by their maxima.
+// and the rows of a short item share its bytes. Waves walk 16 NB keys at a time on their own (no barriers). K fragment: lane (r, g) holds
+// words KT g .. KT g + KT - 1 of key r, one load of 4 KT bytes, and the queries are loaded in that order. V fragment: lane (r, g) takes 4 VH
+// columns of 8 keys; two keys' halves are permuted into one word first, so no transposition is needed. A wave's results, then the
+// workgroups', are merged by their references.
 // Items of up to 8 or 4 columns leave most of the product's 16 unused, and with them most lanes of the softmax: the columns are then given PACK
 // times, and the copies' lanes take the scores of different 16-key blocks, which they have anyhow. Their weights go back to the first copy by
 // moves inside a row of lanes.
+// Measured, 32 heads on 8, 128 wide, bf16: 64 rows behind 8,192 tokens each 107 us, 5.4 TB/s of codes and pairs (a plain read of memory: 6.1); one row
+// of 32 heads behind 131,071 tokens 104 us, 5.5 TB/s. There memory and the vector units, which take a key out of its codes in as many instructions
+// as the products of 16 columns take cycles, are about even. Few keys are bound by a chain of dependent loads (row, slot, page, codes, then the
+// merge's counter): 300 keys 7.3 us, 8 rows behind 4,000 tokens 12.7.
 #include "kv4_attend.h"
 #include "lit_llama_amd.h"
 

@@ -6,6 +6,11 @@
 // this one's products and one barrier a tile is enough. Scores, softmax and weights stay in registers: S^T = K q^T leaves a
 // column's weights where O^T = V^T P^T wants them. Workgroups of one head are 8 apart and so on one XCD, whose L2 holds its pages; items
 // are taken from the last, which see the most keys.
+// Measured, 32 heads on 8, 128 wide: 4,096 rows 220 us, 137 GFLOP of products in 64-key tiles at 0.63 PFLOP/s (a library's bf16 product: 1.17).
+// Instructions of the vector units keep them busy 72 % of the time (softmax 150 a tile and 16 columns, unpacking 110 a tile and wave, at four cycles
+// each), products a quarter; at 32 columns a wave the rest is LDS and barriers. (16 columns a wave and 8 waves, twice the waves on a CU but
+// twice the fragments read: 406 us.) Short prompts are bound by their longest item, 1.6 us a tile alone: six of up to 501 rows, 10 heads of 64 in
+// fp32, 23 us.
 #include <type_traits>
 
 #include "kv4_attend.h"
@@ -16,7 +21,8 @@ namespace llj {
 template <int KT, int VH>
 struct Kv4Tile {
   static constexpr int kKeys = 4 * KT * 1024, kValues = 8 * VH * 1024;  // bytes of unpacked keys, values
-  static constexpr int kPairs = kKeys + kValues, kHere = kPairs + 1024, kBytes = kHere + 16;  // (pairs: key scales, offsets, value scales, offsets; here: 16 keys' page exists)
+  // pairs: key scales, offsets, value scales, offsets as fp32; here: whether the pages of each 16 keys exist
+  static constexpr int kPairs = kKeys + kValues, kHere = kPairs + 1024, kBytes = kHere + 16;
 };
 
 template <typename T, int KT, int VH, int QB>
