@@ -619,7 +619,7 @@ int llj_streams_linear(int act, const void* y, const float* out_w, const float* 
  * values ov, one gate per head at og (-1: none).
  * prep: rotate-half rotation of the first rot_dims dimensions of queries (in place) and keys (turns[i] = frequency of pair
  * (i, i + rot_dims / 2) / 2 pi, doubles), with qk_norm both divided by their root mean square over dim; key and value
- * into the cache (W 0: row m's into row m of it). first (row stride ldf): without lam a copy of the values is left there, with lam the values are
+ * into the cache. first (row stride ldf): without lam a copy of the values is left there, with lam the values are
  * (1 - lam) v + lam first.
  * rows: any sizes; softmax over the row's own and all earlier positions of q . k * scale, with sink one added to the
  * denominator; y = sum p v * sigmoid(gate).
@@ -669,12 +669,17 @@ int llj_pages_release(const int* slot, int B, int* seen, int slots, int* table, 
  * largest bf16 up to the smallest value, s = (largest - o) / 15 rounded to fp32, then bf16, c = (x - o) / s rounded to the nearest
  * (halves to even) and kept in 0 .. 15, all 0 where s is. A vector with an infinity or NaN, or a value below bf16's range, is NaN.
  * write: row m's keys k[m ldk + head hk + i] and values into place[m] (outside the pool: the row is left out; the places of a call differ).
- * read: what stands there, in bf16 or fp32 (outside: zeros). M kv_heads up to 2^26 a call. */
+ * read: what stands there, in bf16 or fp32 (outside: zeros). M kv_heads up to 2^26 a call.
+ * llj_gqa_prep_kv4: llj_gqa_prep whose keys and values go into place[m] in codes, as llj_kv4_write would put them (a row's keys, values and angles
+ * fit 160 KiB; M up to 2^23). */
 size_t llj_kv4_block_bytes(int page, int dim, int vdim);
 int llj_kv4_write(const void* k, size_t ldk, size_t hk, const void* v, size_t ldv, size_t hv, const int* place, int M, int kv_heads, int dim,
                   int vdim, int dt, void* pool, int pages, int page, void* stream);
 int llj_kv4_read(const void* pool, int pages, int page, const int* place, int M, int kv_heads, int dim, int vdim, int dt, void* k, size_t ldk,
                  size_t hk, void* v, size_t ldv, size_t hv, void* stream);
+int llj_gqa_prep_kv4(void* in, int ld, int oq, int ok, int ov, const void* turns, int rot_dims, int qk_norm, float eps, const int* pos,
+                     const int* place, void* pool, int pages, int page, void* first, const float* lam, int ldf, int M, int heads,
+                     int kv_heads, int dim, int vdim, int dt, void* stream);
 /* Grouped-query attention over it: rows q[m ldq + head dim + i], y of stride ldy, gates (NULL: none) of stride ldg. Row m sees the positions up
  * to pos[m] (< 0: none, y = 0; page numbers outside the pool: none of that page) of its sequence's slot; scores q . k * scale, with sink one
  * added to the denominator; y = sum p v * sigmoid(gate). work: `items` (first row, rows, sequence) of at most `rows` rows each (rows not in any

@@ -7,11 +7,14 @@
 //   values     copied beside the cache (first, no lam) or mixed with such a copy, (1 - lam) v + lam first
 //   sink       one is added to the softmax's denominator: a key of score 0 without a value (optional)
 //   gate       head h's output times sigmoid(in[og + h]) (optional, og >= 0)
-// Kernels: row preparation, any-size attention rows (both types), flash prefill and split decode (bf16, MFMA). The
+// Kernels: row preparation (into such rows, or in codes into pages: kv4.h), any-size attention rows (both types), flash prefill and split decode (bf16, MFMA). The
 // decode kernel prepares its own queries and the new key and value. Scores, softmax statistics and weights are
 // fp32; the weights enter the MFMA product as two bf16 terms (p = hi + lo).
+#include <algorithm>
+
 #include "common.h"
 #include "elem.h"
+#include "kv4_rows.h"
 #include "lit_llama_amd.h"
 
 namespace llj {
@@ -27,7 +30,7 @@ struct GqaParams {
   const int* pos;      // position of each row
   const int* row_seq;  // NULL: row m is sequence m
   const int* slot;
-  void* cache;  // [slots][W][ldc]; W 0 (preparation only): [M][ldc]
+  void* cache;  // [slots][W][ldc]
   int W, ldc;
   void* first;  // [M][ldf]
   const float* lam;
@@ -50,13 +53,59 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
 // One row per workgroup: rotation and norm of its queries (in place) and keys (into the cache row), its values. LG
 // lanes share a head; an item is a rotated pair (i, i + RD / 2) or an unrotated dimension (VEC: 8 of them, one item
 // per lane), and belongs to one lane, so the queries' update in place reads nothing another lane writes.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void gqa_prep_kernel(GqaParams p, int LG) {
-  extern __shared__ __attribute__((aligned(16))) float s_cs[];  // [RD / 2] cosines, sines
+// CODES: a workgroup has `heads` K / V heads of a row with their query heads; keys and values stay in LDS, keys before values, and go from there
+// into a paged 4-bit cache. (32 heads on 8 of 128, bf16: one row 4.7 us, preparation and writing one after the other 4.5 + 2.6; 64 rows 5.2, 4.9 +
+// 2.9; 2,048 rows 17.8, 11.7 + 5.6. Bound by a chain: position, angles, barrier, rows, barrier, codes.)
+struct GqaCodes {
+  Kv4Pool pool;
+  const int* place;
+  int heads;
+};
+// n key heads (KEYS) and n value heads (VALUES) from head g0 on, LG lanes each
+template <typename T, int LG, bool KEYS, bool VALUES>
+__device__ __forceinline__ void gqa_codes(const Kv4Pool& pool, const Kv4Part& key, const Kv4Part& val, const T* x, int g0, int n, int place) {
+  const int l = threadIdx.x & (LG - 1);
+  for (int i = threadIdx.x / LG; i < (KEYS && VALUES ? 2 * n : n); i += 256 / LG) {
+    const bool k = KEYS && (!VALUES || i < n);
+    const int g = k ? i : KEYS ? i - n : i;
+    const Kv4Part& part = k ? key : val;
+    const T* at = x + (k ? 0 : n * key.n) + g * part.n;
+    float v[8];
+    if ((key.n | val.n) % 8 == 0) {
+      ld8(at + (8 * l < part.n ? 8 * l : 0), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 8 * l + e < part.n ? ldv(at, 8 * l + e) : 0.f;
+    }
+    kv4_write_row<LG, false>(pool, part, v, l, place, g0 + g);
+  }
+}
+template <typename T, bool KEYS, bool VALUES>
+__device__ __forceinline__ void gqa_codes_any(const Kv4Pool& pool, const Kv4Part& key, const Kv4Part& val, const T* x, int g0, int n, int place) {
+  const int bytes = KEYS ? key.bytes : val.bytes;
+  if (bytes == 32) gqa_codes<T, 8, KEYS, VALUES>(pool, key, val, x, g0, n, place);
+  else if (bytes == 64) gqa_codes<T, 16, KEYS, VALUES>(pool, key, val, x, g0, n, place);
+  else gqa_codes<T, 32, KEYS, VALUES>(pool, key, val, x, g0, n, place);
+}
+
+template <typename T, bool VEC, bool CODES>
+__global__ __launch_bounds__(256) void gqa_prep_kernel(GqaParams p, int LG, GqaCodes codes) {
+  extern __shared__ __attribute__((aligned(16))) float s_cs[];  // [RD / 2] cosines, sines; CODES: the row
   const int m = blockIdx.x, tid = threadIdx.x, n = p.RD / 2, D = p.D;
   T* row = (T*)p.in + (size_t)m * p.ld;
-  const int ps = p.pos[m], b = p.row_seq ? p.row_seq[m] : m;
-  T* dst = (T*)p.cache + (p.W ? (size_t)p.slot[b] * p.W + ps : (size_t)m) * p.ldc;
+  const int ps = p.pos[m], b = p.row_seq ? p.row_seq[m] : m, place = CODES ? codes.place[m] : 0;
+  int g0 = 0;
+  if constexpr (CODES) {  // from here on p is the workgroup's heads
+    g0 = blockIdx.y * codes.heads;
+    const int R = p.H / p.G;
+    p.G = p.G - g0 < codes.heads ? p.G - g0 : codes.heads;
+    p.H = p.G * R;
+    p.oq += g0 * R * D;
+    p.ok += g0 * D;
+    p.ov += g0 * p.V;
+  }
+  T* dst = CODES ? nullptr : (T*)p.cache + ((size_t)p.slot[b] * p.W + ps) * p.ldc;
+  T* s_row = reinterpret_cast<T*>(s_cs + (p.RD + 3) / 4 * 4);
   for (int i = tid; i < n; i += 256) turn_cs(p.turns[i], ps, s_cs[i], s_cs[n + i]);
   __syncthreads();
   const int l = tid & (LG - 1), per = 256 / LG;
@@ -66,7 +115,8 @@ __global__ __launch_bounds__(256) void gqa_prep_kernel(GqaParams p, int LG) {
     const bool live = h < p.H + p.G;
     const bool key = h >= p.H;
     const T* src = row + (key ? p.ok + (live ? h - p.H : 0) * D : p.oq + h * D);
-    T* out = key ? dst + (live ? h - p.H : 0) * D : row + p.oq + h * D;
+    T* out = key && !CODES ? dst + (live ? h - p.H : 0) * D : row + p.oq + h * D;
+    T* lds_out = s_row + (key && live ? h - p.H : 0) * D;
     auto item = [&](int it, float (&a)[E], float (&c)[E]) {  // the values at k, k + n (a pair) or at k
       const bool pair = it < np;
       const int k = pair ? E * it : p.RD + E * (it - np);
@@ -103,24 +153,38 @@ __global__ __launch_bounds__(256) void gqa_prep_kernel(GqaParams p, int LG) {
         a[e] *= r;
         c[e] *= r;
       }
-      if constexpr (VEC) {
-        st8(out + k, a);
-        if (it < np) st8(out + k + n, c);
-      } else {
-        stv(out, k, a[0]);
-        if (it < np) stv(out, k + n, c[0]);
-      }
+      auto put = [&](T* to) {
+        if constexpr (VEC) {
+          st8(to + k, a);
+          if (it < np) st8(to + k + n, c);
+        } else {
+          stv(to, k, a[0]);
+          if (it < np) stv(to, k + n, c[0]);
+        }
+      };
+      if (CODES && key) put(lds_out);
+      else put(out);
     }
   }
   const int GV = p.G * p.V;
-  T* vd = dst + p.G * D;
-  T* fr = p.first ? (T*)p.first + (size_t)m * p.ldf : nullptr;
+  T* vd = CODES ? s_row + p.G * D : dst + p.G * D;
+  T* fr = p.first ? (T*)p.first + (size_t)m * p.ldf + g0 * p.V : nullptr;
   const float lam = p.lam ? *p.lam : 0.f;
   for (int k = tid; k < GV; k += 256) {
     float v = ldv(row, p.ov + k);
     if (p.lam) v = (1.f - lam) * v + lam * ldv(fr, k);
     else if (fr) stv(fr, k, v);
     stv(vd, k, v);
+  }
+  if constexpr (CODES) {
+    __syncthreads();
+    const Kv4Part key = kv4_keys(codes.pool, D), val = kv4_values(codes.pool, p.V);
+    if (key.bytes == val.bytes) {
+      gqa_codes_any<T, true, true>(codes.pool, key, val, s_row, g0, p.G, place);
+    } else {
+      gqa_codes_any<T, true, false>(codes.pool, key, val, s_row, g0, p.G, place);
+      gqa_codes_any<T, false, true>(codes.pool, key, val, s_row, g0, p.G, place);
+    }
   }
 }
 
@@ -692,8 +756,8 @@ __global__ __launch_bounds__(256) void gqa_attend_kernel(GqaParams p, float* par
   }
 }
 
-static int gqa_check(const GqaParams& p, int least = 1) {
-  LLJ_REQUIRE(p.in && p.pos && p.slot && p.cache && p.W >= least && p.M > 0 && p.H > 0 && p.G > 0 && p.H % p.G == 0 && p.D > 0 &&
+static int gqa_check(const GqaParams& p) {
+  LLJ_REQUIRE(p.in && p.pos && p.slot && p.cache && p.W > 0 && p.M > 0 && p.H > 0 && p.G > 0 && p.H % p.G == 0 && p.D > 0 &&
               p.V > 0 && p.ldc >= p.G * (p.D + p.V) && p.oq >= 0 && p.oq + p.H * p.D <= p.ld &&
               (p.og < 0 || p.og + p.H <= p.ld));
   return 0;
@@ -760,6 +824,32 @@ static int gqa_attend_keys(const GqaParams& p, float* part, int* count, int nspl
   return gqa_attend_go<8, DB>(p, part, count, nsplit, sl2, s);
 }
 
+template <typename T, bool CODES>
+static int gqa_prep_go(const GqaParams& p, GqaCodes c, hipStream_t s) {
+  size_t lds = (size_t)(p.RD > 0 ? p.RD : 2) * 4;
+  LLJ_REQUIRE(lds <= 64 * 1024);
+  // few rows: a row's heads over several workgroups, until there are two on a CU (8 K / V heads: a
+  // one-row step of Bobasun 7B 2.97 ms, 3.09 with one workgroup a row)
+  const int parts = CODES ? std::max(1, std::min(p.G, 512 / p.M)) : 1, heads = (p.G + parts - 1) / parts;
+  if (CODES) lds = (size_t)(p.RD + 3) / 4 * 16 + (size_t)heads * (p.D + p.V) * sizeof(T);
+  LLJ_REQUIRE(lds <= 160 * 1024);
+  const int n8 = p.RD / 16 + (p.D - p.RD) / 8;
+  const bool vec = (p.ld | p.oq | p.ok | p.D) % 8 == 0 && p.RD % 16 == 0 && n8 <= 64 && ((uintptr_t)p.in & 15) == 0 &&
+                   (CODES || (p.ldc % 8 == 0 && ((uintptr_t)p.cache & 15) == 0));
+  int lg = 64;
+  if (vec)
+    while (lg > 1 && lg / 2 >= n8) lg /= 2;
+  auto kern = vec ? gqa_prep_kernel<T, true, CODES> : gqa_prep_kernel<T, false, CODES>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  c.heads = heads;
+  hipLaunchKernelGGL(kern, dim3(p.M, (p.G + heads - 1) / heads), dim3(256), lds, s, p, lg, c);
+  LLJ_CHECK_LAUNCH();
+  return 0;
+}
+
 }  // namespace llj
 
 using namespace llj;
@@ -776,26 +866,24 @@ int llj_gqa_prep(void* in, int ld, int oq, int ok, int ov, const void* turns, in
   p.pos = pos; p.row_seq = row_seq; p.slot = slot; p.cache = cache; p.W = W; p.ldc = ldc;
   p.first = first; p.lam = lam; p.ldf = ldf; p.M = M; p.H = heads; p.G = kv_heads; p.D = dim; p.V = vdim;
   LLJ_REQUIRE(dt == 0 || dt == 1);
-  if (const int rc = gqa_check(p, 0)) return rc;
+  if (const int rc = gqa_check(p)) return rc;
   if (const int rc = gqa_check_new(p)) return rc;
-  const size_t lds = (size_t)(rot_dims > 0 ? rot_dims : 2) * 4;
-  LLJ_REQUIRE(lds <= 64 * 1024);
-  const int n8 = rot_dims / 16 + (dim - rot_dims) / 8;
-  const bool vec = (ld | oq | ok | dim | ldc) % 8 == 0 && rot_dims % 16 == 0 && n8 <= 64 &&
-                   (((uintptr_t)in | (uintptr_t)cache) & 15) == 0;
-  int lg = 64;
-  if (vec)
-    while (lg > 1 && lg / 2 >= n8) lg /= 2;
-  hipStream_t s = (hipStream_t)stream;
-#define LLJ_GP(T)                                                                                          \
-  do {                                                                                                     \
-    if (vec) hipLaunchKernelGGL((gqa_prep_kernel<T, true>), dim3(M), dim3(256), lds, s, p, lg);            \
-    else hipLaunchKernelGGL((gqa_prep_kernel<T, false>), dim3(M), dim3(256), lds, s, p, lg);               \
-  } while (0)
-  LLJ_DT(dt, LLJ_GP(bf16_t), LLJ_GP(float));
-#undef LLJ_GP
-  LLJ_CHECK_LAUNCH();
-  return 0;
+  return dt == 0 ? gqa_prep_go<bf16_t, false>(p, {}, (hipStream_t)stream) : gqa_prep_go<float, false>(p, {}, (hipStream_t)stream);
+}
+
+int llj_gqa_prep_kv4(void* in, int ld, int oq, int ok, int ov, const void* turns, int rot_dims, int qk_norm, float eps, const int* pos,
+                     const int* place, void* pool, int pages, int page, void* first, const float* lam, int ldf, int M, int heads,
+                     int kv_heads, int dim, int vdim, int dt, void* stream) {
+  LLJ_REQUIRE(kv4_sizes(pool, pages, page, kv_heads, dim, vdim, dt) && place && heads >= 1 && heads <= 65535 && M <= 1 << 23);
+  GqaParams p{};
+  p.in = in; p.ld = ld; p.oq = oq; p.ok = ok; p.ov = ov; p.og = -1;
+  p.turns = (const double*)turns; p.RD = rot_dims; p.qk_norm = qk_norm; p.eps = eps;
+  p.pos = pos; p.first = first; p.lam = lam; p.ldf = ldf; p.M = M; p.H = heads; p.G = kv_heads; p.D = dim; p.V = vdim;
+  p.slot = pos; p.cache = pool; p.W = 1; p.ldc = kv_heads * (dim + vdim);  // (of rows in LDS: neither is read)
+  if (const int rc = gqa_check(p)) return rc;
+  if (const int rc = gqa_check_new(p)) return rc;
+  const GqaCodes c{kv4_pool(pool, pages, kv_heads, kv4_page_log2(page), dim, vdim), place, 0};
+  return dt == 0 ? gqa_prep_go<bf16_t, true>(p, c, (hipStream_t)stream) : gqa_prep_go<float, true>(p, c, (hipStream_t)stream);
 }
 
 int llj_gqa_rows(const void* in, int ld, int oq, int og, const int* pos, const int* row_seq, const int* slot, const void* cache,

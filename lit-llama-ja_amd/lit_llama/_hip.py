@@ -157,6 +157,7 @@ SIGNATURES = {
     "llj_pages_release": [_P, _I, _P, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P],
     "llj_kv4_write": [_P, _U64, _U64, _P, _U64, _U64, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P],
     "llj_kv4_read": [_P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _U64, _U64, _P, _U64, _U64, _P],
+    "llj_gqa_prep_kv4": [_P, _I, _I, _I, _I, _P, _I, _I, _F, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "llj_kv4_part_width": [_I],
     "llj_kv4_tiles": [_I, _I, _I, _I, _I, _I],
     "llj_kv4_attend": [_P, _I, _P, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I,

@@ -431,7 +431,11 @@ class GroupedAttention:
 
     def cache_layout(self, page: int) -> kv4.Layout:
         """The layer's keys and values in 4 bits."""
-        return kv4.Layout(self.spec.kv_heads, self.spec.dim, self.spec.vdim, page)
+        s = self.spec
+        row = 4 * s.rot_dims + 16 + s.kv_heads * (s.dim + s.vdim) * self.dtype.itemsize
+        if row > 160 * 1024:  # (llj_gqa_prep_kv4 forms a row's codes from shared memory)
+            raise ValueError(f"{s.kv_heads} heads of {s.dim} + {s.vdim}: {row} bytes of keys and values a row, {160 * 1024} at most in 4 bits")
+        return kv4.Layout(s.kv_heads, s.dim, s.vdim, page)
 
     def out_width(self) -> int:
         return self.spec.heads * self.spec.vdim
@@ -497,16 +501,14 @@ class GroupedAttention:
 
 
     def _mix_int4(self, i: int, rows, w, state, y: torch.Tensor, st) -> None:
-        """mix() over a cache in 4 bits (state.extend's places for the call's rows are in rows.pages): rotation and norm of queries and keys
-        into a row of their own, codes into the pages, attention over those."""
+        """mix() over a cache in 4 bits (state.extend's places for the call's rows are in rows.pages): rotation and norm of queries and keys,
+        keys and values into the pages in codes, attention over those."""
         s, p, o, M = self.spec, w.proj, self.inp.offset, rows.M
-        layout, ldc, GD = state.layout[i], self.cache_width(self.dtype), s.kv_heads * s.dim
+        layout, pool = state.layout[i], state.pool[i]
         first = w.first if s.v_mix else None
-        kv = w.buffer("kv", M * ldc, self.dtype)[:M * ldc].view(M, ldc)
-        _hip.call("llj_gqa_prep", p.data_ptr(), p.stride(0), o[0], o[1], o[2], self.turns.data_ptr(), s.rot_dims, int(s.qk_norm), self.eps,
-                  rows.pos.data_ptr(), _hip.ptr(rows.row_seq), rows.slot.data_ptr(), kv.data_ptr(), 0, ldc, _hip.ptr(first), _hip.ptr(self.lam),
+        _hip.call("llj_gqa_prep_kv4", p.data_ptr(), p.stride(0), o[0], o[1], o[2], self.turns.data_ptr(), s.rot_dims, int(s.qk_norm), self.eps,
+                  rows.pos.data_ptr(), rows.pages.place.data_ptr(), pool.data_ptr(), pool.shape[0], layout.page, _hip.ptr(first), _hip.ptr(self.lam),
                   0 if first is None else first.stride(0), M, s.heads, s.kv_heads, s.dim, s.vdim, _dt(self.dtype), st)
-        kv4.write(state.pool[i], layout, kv[:, :GD], kv[:, GD:GD + s.kv_heads * s.vdim], rows.pages.place)
         per, work = 1, None
         if not rows.decode:
             per = kv4.item_rows(layout, s.heads, max(rows.lengths), self.dtype)
@@ -514,7 +516,7 @@ class GroupedAttention:
             work = work.view(n, 3)
         n, need = kv4.splits(layout, s.heads, M if work is None else n, per, state.table.shape[1] * layout.page, self.dtype)
         count = w.buffer("count4", need, torch.int32, zero=True) if n > 1 and need else None
-        kv4.attend(p[:M, o[0]:o[0] + s.heads * s.dim], state.pool[i], layout, state.table, rows.slot, rows.pages.pos, work=work, rows=per, scale=s.scale,
+        kv4.attend(p[:M, o[0]:o[0] + s.heads * s.dim], pool, layout, state.table, rows.slot, rows.pages.pos, work=work, rows=per, scale=s.scale,
                    sink=s.sink, gate=p[:M, o[3]:o[3] + s.heads], out=y[:M, :s.heads * s.vdim], count=count)
 
 

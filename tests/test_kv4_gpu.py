@@ -140,6 +140,51 @@ def test_strides_and_places_outside(hip, dtype):
     assert same(b.double().cpu().numpy(), O.stands_for(gaps[:, :, 1 + D:]).astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,D,V,RD,norm,mix", [(4, 2, 64, 64, 64, 1, None), (8, 2, 128, 128, 32, 1, "copy"), (6, 3, 78, 78, 10, 0, "mix"), (5, 1, 40, 200, 0, 1, "mix"),
+                                                 (3, 3, 256, 130, 256, 1, None), (4, 4, 33, 17, 2, 1, "copy"), (40, 10, 64, 64, 64, 1, "mix"), (2, 1, 8, 1, 8, 0, None),
+                                                 (64, 64, 256, 256, 64, 1, None)])
+def test_prepared_rows(hip, dtype, H, G, D, V, RD, norm, mix):
+    """llj_gqa_prep_kv4: the pool's bytes, the queries and the values kept aside are those of llj_gqa_prep into plain rows and write out of them. Rows
+    without a place prepare their queries all the same. 64 fp32 heads of 256 + 256 (256 KiB a row) are refused."""
+    from lit_llama import _hip, kv4
+
+    g = np.random.default_rng(H + D)
+    M, page = 19, 32
+    oq, ok, ov, ld = 8, 8 + H * D, 16 + (H + G) * D, 24 + (H + G) * D + G * V
+    ld += -ld % 8
+    _, x = rounded(g.standard_normal((M, ld)), dtype)
+    _, f0 = rounded(g.standard_normal((M, G * V + 3)), dtype)
+    lam = torch.tensor([0.3], device="cuda")
+    turns = torch.tensor(g.random(max(RD // 2, 1)), dtype=torch.float64, device="cuda")
+    pos, slot = ints(g.integers(0, 64, M)), ints(range(M))
+    place = g.permutation(5 * page)[:M]
+    place[4], place[11] = -1, 5 * page
+    place, lay, dt = ints(place), kv4.Layout(G, D, V, page), 0 if dtype == torch.bfloat16 else 1
+    out = []
+    for fused in (False, True):
+        y, f, pool = x.clone(), f0.clone(), lay.pool(5)
+        head = (y.data_ptr(), ld, oq, ok, ov, turns.data_ptr(), RD, norm, 1e-5)
+        keep = (f.data_ptr() if mix else None, lam.data_ptr() if mix == "mix" else None, f.stride(0))
+        tail = (M, H, G, D, V, dt, _hip.stream())
+        if fused:
+            args = (*head, pos.data_ptr(), place.data_ptr(), pool.data_ptr(), 5, page, *keep, *tail)
+            if G * (D + V) * dtype.itemsize > 160 * 1024 - 4 * RD:
+                with pytest.raises(_hip.HipError):
+                    _hip.call("llj_gqa_prep_kv4", *args)
+                return
+            _hip.call("llj_gqa_prep_kv4", *args)
+        else:
+            ldc = -(-G * (D + V) // 8) * 8
+            cache = torch.empty(M, 64, ldc, dtype=dtype, device="cuda")
+            _hip.call("llj_gqa_prep", *head, pos.data_ptr(), None, slot.data_ptr(), cache.data_ptr(), 64, ldc, *keep, *tail)
+            kv = cache[torch.arange(M, device="cuda"), pos.long()]
+            kv4.write(pool, lay, kv[:, :G * D], kv[:, G * D:G * (D + V)], place)
+        out.append((y, f, pool))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------------------- attention
 class Case:
     """Sequences of `lens` tokens in scattered pages; the last rows[b] of each are the rows of the call (0: none)."""

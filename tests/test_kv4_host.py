@@ -108,6 +108,17 @@ def test_rows_refuse():
     assert lib().llj_kv4_write(*{**good, "M": 0}.values()) == 0
 
 
+def test_preparation_refuses():
+    good = dict(inp=P, ld=256, oq=0, ok=128, ov=192, turns=P, rot=32, norm=1, eps=1e-5, pos=P, place=P, pool=P, pages=4, page=16, first=None, lam=None,
+                ldf=0, M=3, heads=4, kv_heads=2, dim=32, vdim=32, dt=0, stream=None)
+    bad = [dict(inp=None), dict(ld=255), dict(oq=-1), dict(ok=200), dict(ov=193), dict(turns=None), dict(rot=33), dict(rot=34), dict(pos=None),
+           dict(place=None), dict(pool=None), dict(pool=P + 8), dict(pages=0), dict(page=24), dict(lam=P), dict(first=P, ldf=63), dict(M=0),
+           dict(M=(1 << 23) + 1), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(vdim=0), dict(vdim=300), dict(dt=2),
+           dict(heads=200, kv_heads=200, dim=256, vdim=256, ld=1 << 20, ok=1 << 18, ov=1 << 19)]
+    for b in bad:
+        assert lib().llj_gqa_prep_kv4(*{**good, **b}.values()) == EINVAL, b
+
+
 def test_attention_refuses():
     good = dict(q=P, ldq=256, gate=None, ldg=0, work=P, items=2, rows=2, pos=P, slot=P, B=2, table=P, slots=4, ldt=8, pool=P, pages=4, page=16, part=P,
                 count=P, nsplit=2, y=P, ldy=256, M=4, heads=4, kv_heads=2, dim=64, vdim=64, scale=1.0, sink=0, dt=0, stream=None)
