@@ -831,8 +831,11 @@ static int gqa_prep_go(const GqaParams& p, GqaCodes c, hipStream_t s) {
   // few rows: a row's heads over several workgroups, until there are two on a CU (8 K / V heads: a
   // one-row step of Bobasun 7B 2.97 ms, 3.09 with one workgroup a row)
   const int parts = CODES ? std::max(1, std::min(p.G, 512 / p.M)) : 1, heads = (p.G + parts - 1) / parts;
-  if (CODES) lds = (size_t)(p.RD + 3) / 4 * 16 + (size_t)heads * (p.D + p.V) * sizeof(T);
-  LLJ_REQUIRE(lds <= 160 * 1024);
+  if (CODES) {
+    lds = (size_t)(p.RD + 3) / 4 * 16;
+    LLJ_REQUIRE(lds + (size_t)p.G * (p.D + p.V) * sizeof(T) <= 160 * 1024);  // (whatever the rows: of all heads)
+    lds += (size_t)heads * (p.D + p.V) * sizeof(T);
+  }
   const int n8 = p.RD / 16 + (p.D - p.RD) / 8;
   const bool vec = (p.ld | p.oq | p.ok | p.D) % 8 == 0 && p.RD % 16 == 0 && n8 <= 64 && ((uintptr_t)p.in & 15) == 0 &&
                    (CODES || (p.ldc % 8 == 0 && ((uintptr_t)p.cache & 15) == 0));

@@ -143,10 +143,10 @@ def test_strides_and_places_outside(hip, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,G,D,V,RD,norm,mix", [(4, 2, 64, 64, 64, 1, None), (8, 2, 128, 128, 32, 1, "copy"), (6, 3, 78, 78, 10, 0, "mix"), (5, 1, 40, 200, 0, 1, "mix"),
                                                  (3, 3, 256, 130, 256, 1, None), (4, 4, 33, 17, 2, 1, "copy"), (40, 10, 64, 64, 64, 1, "mix"), (2, 1, 8, 1, 8, 0, None),
-                                                 (64, 64, 256, 256, 64, 1, None)])
+                                                 (64, 64, 256, 256, 64, 1, None), (96, 96, 256, 256, 64, 1, None)])
 def test_prepared_rows(hip, dtype, H, G, D, V, RD, norm, mix):
     """llj_gqa_prep_kv4: the pool's bytes, the queries and the values kept aside are those of llj_gqa_prep into plain rows and write out of them. Rows
-    without a place prepare their queries all the same. 64 fp32 heads of 256 + 256 (256 KiB a row) are refused."""
+    without a place prepare their queries all the same. 96 fp32 heads of 256 + 256 (192 KiB a row) are refused."""
     from lit_llama import _hip, kv4
 
     g = np.random.default_rng(H + D)
@@ -181,6 +181,29 @@ def test_prepared_rows(hip, dtype, H, G, D, V, RD, norm, mix):
             kv = cache[torch.arange(M, device="cuda"), pos.long()]
             kv4.write(pool, lay, kv[:, :G * D], kv[:, G * D:G * (D + V)], place)
         out.append((y, f, pool))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G,D,V", [(64, 256, 256), (7, 64, 96), (16, 130, 20)])
+def test_prepared_rows_in_one_workgroup_each(hip, dtype, G, D, V):
+    """520 rows of a call, whose heads stay in one workgroup (128 KiB of keys and values in fp32), against calls of 8 rows, whose heads are spread."""
+    from lit_llama import _hip, kv4
+
+    g = np.random.default_rng(G)
+    M, page, H = 520, 64, 2 * G
+    ld = (H + G) * D + G * V
+    _, x = rounded(g.standard_normal((M, ld)), dtype)
+    turns = torch.tensor(g.random(16), dtype=torch.float64, device="cuda")
+    pos, place, lay, dt = ints(range(M)), ints(g.permutation(9 * page)[:M]), kv4.Layout(G, D, V, page), 0 if dtype == torch.bfloat16 else 1
+    out = []
+    for n in (520, 8):
+        y, pool = x.clone(), lay.pool(9)
+        for m in range(0, M, n):
+            _hip.call("llj_gqa_prep_kv4", y[m:].data_ptr(), ld, 0, H * D, (H + G) * D, turns.data_ptr(), 32, 1, 1e-5, pos[m:].data_ptr(), place[m:].data_ptr(),
+                      pool.data_ptr(), 9, page, None, None, 0, n, H, G, D, V, dt, _hip.stream())
+        out.append((y, pool))
     for a, b in zip(*out):
         assert torch.equal(a, b)
 
