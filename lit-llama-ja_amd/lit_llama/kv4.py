@@ -18,10 +18,15 @@ from .pages import PAGE_SIZES, ints, on_device
 # Key ranges of a call, at most. Few rows: a range is at least a round of its workgroup's waves, from 16 ranges on two (one sequence of 16,000 keys, 8
 # K / V heads: 32 ranges 14.2 us, 64 18.0; of 4,000: 16 ranges 10.1, 4 12.7), and 512 workgroups or, of ranges of 1,024 keys, three on a CU (24 sequences
 # of 4,000: 4 ranges 24.5 us, 2 26.4, one 29.5; 32 of 8,000: 3 ranges 49.2, one 54.6; 32 of 2,000: 2 ranges 19.3, one 18.8, 4 21.0). A sequence
-# that is shorter than the table allows takes fewer by itself. Prompt rows, whose ranges are put together by a launch of
-# their own: 1,024 keys (512 rows behind 60,000 tokens: 4 ranges 703 us, one 1,925; 512 rows of a prompt alone: one 25.9, two 28.4).
+# that is shorter than the table allows takes fewer by itself.
+# Prompt rows: a tile of 64 keys takes TILE us (half as much again with two workgroups on a CU), and ranges a launch of JOIN us that reads what they wrote at
+# PART bytes a us, there and back, and RANGE_STEP us more a range. The sum over n ranges is least at the root of TILE tiles / (what a range costs),
+# measured within a tenth of the best of 12 numbers in 13 of 14 calls (512 rows behind 60,000 tokens: 4 ranges 688 us, one 1,974; 128 rows of 8
+# heads' keys behind 2,048: 7 ranges 28, two 47, one 76; 24 rows of 20 fp32 heads on one behind 9,400: 31 ranges 33, 10 47; 512 rows of a
+# prompt alone: one 25.9, two 28.4).
 WGS, WGS_LONG = 512, 768
 RANGE, RANGES, RANGE_LONG = 256, 16, 1024
+TILE, JOIN, RANGE_STEP, PART = 2.2, 8.0, 0.2, 4e6
 FEW_COLUMNS = 64  # (row, head) pairs of a K / V head in an item: from more on it is prompt rows (csrc/kv4_attend.hip)
 
 
@@ -34,6 +39,11 @@ def _block_bytes(page: int, dim: int, vdim: int) -> int:
 @lru_cache(4096)
 def _tiles(heads: int, kv_heads: int, dim: int, vdim: int, rows: int, dt: int) -> int:
     return int(_hip.lib().llj_kv4_tiles(heads, kv_heads, dim, vdim, rows, dt))
+
+
+@lru_cache(None)
+def _part_bytes(vdim: int) -> int:
+    return 4 * int(_hip.lib().llj_kv4_part_width(vdim))
 
 
 def _dt(t: torch.dtype) -> int:
@@ -137,22 +147,33 @@ def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: 
     tiles = _tiles(heads, layout.kv_heads, layout.dim, layout.vdim, rows, _dt(dtype))
     if not tiles:
         raise ValueError(f"{heads} heads on {layout.kv_heads}, items of {rows} rows")
-    wgs, long = max(1, items * tiles), -(-keys // RANGE_LONG)
+    wgs = max(1, items * tiles)
     if rows * heads // layout.kv_heads > FEW_COLUMNS:
-        return max(1, min(64, long, WGS // wgs)), 0
+        return _prompt_splits(wgs, -(-keys // 64), rows * heads / tiles * _part_bytes(layout.vdim) * 2 / PART), 0
+    long = -(-keys // RANGE_LONG)
     n = -(-keys // RANGE)
     if n > RANGES:
         n = max(RANGES, -(-keys // (2 * RANGE)))
     return max(1, min(64, max(min(n, WGS // wgs), min(long, WGS_LONG // wgs)))), items * tiles
 
 
-def item_rows(layout: Layout, heads: int, longest: int, dtype: torch.dtype) -> int:
+def _prompt_splits(wgs: int, tiles: int, part: float) -> int:
+    """Key ranges of wgs workgroups over so many tiles, whose parts take `part` us a range."""
+    most = min(64, tiles, WGS // wgs)
+    if most < 2:
+        return 1
+    each = RANGE_STEP + wgs * part
+    n = max(1, min(most, round((TILE * tiles / each) ** 0.5)))
+    left = -(-tiles // n) * (1.0 if wgs * n <= 256 else 1.5)
+    return n if TILE * (tiles - left) > JOIN + each * n else 1
+
+
+def item_rows(layout: Layout, heads: int, longest: int) -> int:
     """Rows of a work item for sequences of up to `longest` rows in a call: few rows share the 16 columns of a tile, prompt rows the
-    128 (fp32 rows and heads over 128: 64) that a tile of keys is unpacked for."""
+    128 that a tile of keys is unpacked for (fp32 rows and heads over 128 in two tiles of 64; items of 64, which are few rows, took 713 us
+    for 394 at 4,096 fp32 rows of 32 heads on 8)."""
     R = heads // layout.kv_heads
-    if longest * R <= FEW_COLUMNS:
-        return max(1, 16 // R)
-    return max(1, (128 if dtype == torch.bfloat16 and max(layout.dim, layout.vdim) <= 128 else 64) // R)
+    return max(1, (16 if longest * R <= FEW_COLUMNS else 128) // R)
 
 
 def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Tensor, slot: torch.Tensor, pos: torch.Tensor, *,
@@ -195,7 +216,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Ten
     n, need = splits(layout, H, items, rows, width * page, dtype)
     part_at = counters = None
     if n > 1:
-        part = torch.empty(M * H * n * _hip.lib().llj_kv4_part_width(V), dtype=torch.float32, device=q.device)
+        part = torch.empty(M * H * n * _part_bytes(V) // 4, dtype=torch.float32, device=q.device)
         part_at = part.data_ptr()
         if need:
             if count is None:

@@ -511,7 +511,7 @@ class GroupedAttention:
                   0 if first is None else first.stride(0), M, s.heads, s.kv_heads, s.dim, s.vdim, _dt(self.dtype), st)
         per, work = 1, None
         if not rows.decode:
-            per = kv4.item_rows(layout, s.heads, max(rows.lengths), self.dtype)
+            per = kv4.item_rows(layout, s.heads, max(rows.lengths))
             n, work, _ = rows.chunks(per)
             work = work.view(n, 3)
         n, need = kv4.splits(layout, s.heads, M if work is None else n, per, state.table.shape[1] * layout.page, self.dtype)

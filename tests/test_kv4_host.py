@@ -77,6 +77,10 @@ def test_tiles_and_ranges():
     for items, keys in ((1, 10), (1, 300), (1, 1 << 20), (8, 4096), (64, 8192), (4096, 1 << 20)):
         n, need = kv4.splits(lay, 32, items, 1, keys)
         assert 1 <= n <= 64 and (n == 1 or n * kv4.RANGE < keys + kv4.RANGE) and need == items * 8
+    for items, rows, keys in ((1, 32, 64), (1, 32, 1000), (1, 17, 1 << 20), (16, 32, 512), (16, 32, 60000), (64, 32, 4096), (5000, 200, 1 << 20)):
+        n, need = kv4.splits(lay, 32, items, rows, keys)
+        assert 1 <= n <= min(64, -(-keys // 64)) and need == 0 and (n == 1 or n * items * 8 <= kv4.WGS)
+    assert kv4.splits(lay, 32, 1, 32, 1 << 20)[0] == 64 and kv4.splits(lay, 32, 16, 32, 512)[0] == 1
 
 
 P = 4096  # an address that nothing is read from: the calls below end at their checks
@@ -175,6 +179,8 @@ def test_rows_of_an_item():
     from lit_llama import kv4
 
     lay = kv4.Layout(8, 128, 128, 64)
-    assert kv4.item_rows(lay, 32, 1, torch.bfloat16) == 4 and kv4.item_rows(lay, 32, 16, torch.bfloat16) == 4
-    assert kv4.item_rows(lay, 32, 17, torch.bfloat16) == 32 and kv4.item_rows(lay, 32, 17, torch.float32) == 16
-    assert kv4.item_rows(kv4.Layout(1, 200, 64, 16), 20, 500, torch.bfloat16) == 3 and kv4.item_rows(kv4.Layout(1, 64, 64, 16), 300, 1, torch.float32) == 1
+    assert [kv4.item_rows(lay, 32, n) for n in (1, 16, 17, 5000)] == [4, 4, 32, 32]
+    assert kv4.item_rows(kv4.Layout(1, 200, 64, 16), 20, 500) == 6 and kv4.item_rows(kv4.Layout(1, 64, 64, 16), 300, 1) == 1
+    for heads in range(1, 301):  # prompt rows' items are prompt rows
+        per = kv4.item_rows(kv4.Layout(1, 64, 64, 16), heads, 1000)
+        assert per * heads > kv4.FEW_COLUMNS and (per * heads <= 128 or per == 1)
