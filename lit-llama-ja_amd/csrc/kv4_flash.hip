@@ -6,7 +6,7 @@
 // this one's products and one barrier a tile is enough. Scores, softmax and weights stay in registers: S^T = K q^T leaves a
 // column's weights where O^T = V^T P^T wants them. Workgroups of one head are 8 apart and so on one XCD, whose L2 holds its pages; items
 // are taken from the last, which see the most keys.
-// Measured, 32 heads on 8, 128 wide: 4,096 rows 220 us, 137 GFLOP of products in 64-key tiles at 0.63 PFLOP/s (a library's bf16 product: 1.17).
+// Measured, 32 heads on 8, 128 wide: 4,096 rows 216 us, 137 GFLOP of products in 64-key tiles at 0.64 PFLOP/s (a library's bf16 product: 1.17).
 // Instructions of the vector units keep them busy 72 % of the time (softmax 150 a tile and 16 columns, unpacking 110 a tile and wave, at four cycles
 // each), products a quarter; at 32 columns a wave the rest is LDS and barriers. (16 columns a wave and 8 waves, twice the waves on a CU but
 // twice the fragments read: 406 us.) Short prompts are bound by their longest item, 1.6 us a tile alone: six of up to 501 rows, 10 heads of 64 in
@@ -207,7 +207,9 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
       if (c + 1 < KT / 2) keys(c + 1);
       __builtin_amdgcn_sched_barrier(0);
       if (c == 0) unpack(then);
+      __builtin_amdgcn_s_setprio(1);  // (products before the other wave's vector work, which runs beside them: 4,096 rows 216 us, 221 without)
       products(c);
+      __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -314,10 +316,13 @@ __global__ __launch_bounds__(256, KT <= 4 && VH <= 2 ? 2 : 1) void kv4_flash_ker
     values(0);  // (the scores' registers are free now)
     values(1);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int q = 0; q < QB; ++q) add(q, u, pt[q]);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
   }
   // ---- lane (col, g) holds values VW / 4 g + 4 VH i + 4 v + d of its columns
