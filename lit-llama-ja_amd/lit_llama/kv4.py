@@ -135,8 +135,8 @@ def read(pool: torch.Tensor, layout: Layout, place: torch.Tensor, dtype: torch.d
     index, pages = _pool(pool, layout)
     M, dt = ints(place, "place", 1, index), _dt(dtype)
     G, D, V = layout.kv_heads, layout.dim, layout.vdim
-    k = torch.empty(M, G, D, dtype=dtype, device=pool.device)
-    v = torch.empty(M, G, V, dtype=dtype, device=pool.device)
+    k = pool.new_empty(M, G, D, dtype=dtype)
+    v = pool.new_empty(M, G, V, dtype=dtype)
     _hip.call_on(index, "llj_kv4_read", pool.data_ptr(), pages, layout.page, place.data_ptr(), M, G, D, V, dt, k.data_ptr(), G * D, D, v.data_ptr(),
                  G * V, V)
     return k, v
@@ -150,6 +150,8 @@ def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: 
     wgs = max(1, items * tiles)
     if rows * heads // layout.kv_heads > FEW_COLUMNS:
         return _prompt_splits(wgs, -(-keys // 64), rows * heads / tiles * _part_bytes(layout.vdim) * 2 / PART), 0
+    if keys <= (2 if max(layout.dim, layout.vdim) <= 128 else 1) * RANGE:  # (two rounds of four waves: the device makes one range of it)
+        return 1, items * tiles
     long = -(-keys // RANGE_LONG)
     n = -(-keys // RANGE)
     if n > RANGES:
@@ -206,7 +208,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Ten
         if work.size(1) != 3 or rows < 1:
             raise ValueError("work items are (first row, rows, sequence), of at least one row")
     if out is None:
-        out = torch.empty(M, H * V, dtype=dtype, device=q.device)
+        out = q.new_empty(M, H * V)
         ldo = H * V
     else:
         ldo = _lead(out, "out", M, H * V, index)
@@ -216,7 +218,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, layout: Layout, table: torch.Ten
     n, need = splits(layout, H, items, rows, width * page, dtype)
     part_at = counters = None
     if n > 1:
-        part = torch.empty(M * H * n * _part_bytes(V) // 4, dtype=torch.float32, device=q.device)
+        part = pool.new_empty(M * H * n * _part_bytes(V))
         part_at = part.data_ptr()
         if need:
             if count is None:

@@ -89,7 +89,7 @@ def extend(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: t
     n = M // chunk + B if chunk else 0
     if n > 1 << 28:
         raise ValueError(f"{n} work items")
-    o = torch.empty(3 * M + 3 * n + 3 * B + 4, dtype=torch.int32, device=table.device)
+    o = table.new_empty(3 * M + 3 * n + 3 * B + 4)
     row_seq, pos, place, work, row0, item0, after, left, status = o.split_with_sizes([M, M, M, 3 * n, B + 1, B + 1, B, 1, 1])
     rows = o.data_ptr()
     items = rows + 12 * M
@@ -107,7 +107,7 @@ def release(table: torch.Tensor, seen: torch.Tensor, free: torch.Tensor, nfree: 
     index, slots, width, B, cap = _tables(table, seen, free, nfree, slot, page)
     if fault is not None and ints(fault, "fault", 1, index) != 1:
         raise ValueError("fault is one int32")
-    status = torch.empty(1, dtype=torch.int32, device=table.device)
+    status = table.new_empty(1)
     _hip.call_on(index, "llj_pages_release", slot.data_ptr(), B, seen.data_ptr(), slots, table.data_ptr(), width, free.data_ptr(), nfree.data_ptr(),
                  cap, page, status.data_ptr(), _hip.ptr(fault))
     return status
