@@ -11,7 +11,7 @@
 // Measured, 32 heads on 8, 128 wide, bf16: 64 rows behind 8,192 tokens each 107 us, 5.4 TB/s of codes and pairs (a plain read of memory: 6.1); one row
 // of 32 heads behind 131,071 tokens 104 us, 5.5 TB/s. There memory and the vector units, which take a key out of its codes in as many instructions
 // as the products of 16 columns take cycles, are about even. Few keys are bound by a chain of dependent loads (row, slot, page, codes, then the
-// merge's counter): 300 keys 7.3 us, 8 rows behind 4,000 tokens 12.7.
+// merge's counter): 300 keys 7.2 us, 8 rows behind 4,000 tokens 12.5.
 #include "kv4_attend.h"
 #include "lit_llama_amd.h"
 

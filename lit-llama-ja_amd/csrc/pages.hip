@@ -11,7 +11,7 @@
 // The sums run in one workgroup (a call has at most kMaxSeqs sequences, whose sums stay in LDS), so nothing of the tables is handed from one
 // workgroup to another inside a launch. Everything else is a flat loop over pages, rows or work items, each of which finds
 // its sequence by bisection. Bound by the chain of dependent loads (slot, length, page, place), not by bytes: a step of 8 sequences 3.8 us, 48
-// sequences with 9 prompts of 6,400 rows 6.7 and 4.0 (rows), 2,048 sequences 8.9 and 5.5.
+// sequences with 9 prompts of 6,400 rows 9.4, 2,048 sequences with 130,000 rows 8.9 and 5.5 (rows).
 #include "common.h"
 #include "lit_llama_amd.h"
 
@@ -22,7 +22,7 @@ constexpr int kMaxSlots = 65536;  // a bit each in LDS
 constexpr int kPlanThreads = 1024;
 constexpr int kSat = 0x3fffffff;  // sums saturate here: past every size that is taken
 constexpr int kMaxTokens = 1 << 30;  // of a sequence
-constexpr int kFewRows = 4096;    // calls up to this many rows and items are one launch
+constexpr int kFewRows = 8192;    // calls up to this many rows and items are one launch (6,400 rows: 9.4 us, in two launches 6.7 + 4.1)
 
 struct ExtendParams {
   const int *slot, *add;

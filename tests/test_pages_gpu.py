@@ -84,7 +84,7 @@ def test_many_sequences(hip, B):
     t.check(slots, [1] * B, ones=True, extra=1)
 
 
-@pytest.mark.parametrize("M", [4095, 4096, 4097, 30000])
+@pytest.mark.parametrize("M", [4095, 4096, 4097, 8191, 8192, 8193, 30000])
 def test_long_prompts(hip, M):
     """On both sides of the size from which the rows have a launch of their own."""
     t = Both(4, 4000, 8000, 16)
