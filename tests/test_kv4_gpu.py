@@ -487,6 +487,28 @@ def test_pages_far_into_a_large_pool(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [128, 256])
+def test_wide_heads_in_a_graph(hip, dtype, D):
+    """Kernels of more than 64 KiB of shared memory, never launched before the capture of their call: a step and prompt rows."""
+    c = Case([700, 300], [1, 1], 4, 2, D, D, 64, dtype, seed=D)
+    p = Case([200], [150], 4, 2, D, D, 64, dtype, seed=D + 1)
+    work, pos, ppos, graph = p.work(64), ints(c.pos), ints(p.pos), torch.cuda.CUDAGraph()
+    from lit_llama import kv4
+
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = kv4.attend(c.qd, c.pool, c.lay, c.table, c.slot, pos)
+        z = kv4.attend(p.qd, p.pool, p.lay, p.table, p.slot, ppos, work=work, rows=64)
+    for _ in range(3):
+        y.fill_(7.0)
+        z.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(y)
+        p.check(z)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_prompt_rows_in_a_graph(hip, dtype):
     """Rows behind a long cache, in key ranges that a second launch joins, captured and replayed over new queries and lengths."""
     from lit_llama import kv4
