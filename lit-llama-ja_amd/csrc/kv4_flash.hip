@@ -390,9 +390,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attend p) {
 constexpr int kv4_blocks(int D, int V, int dt) { return dt == 0 && D <= 128 && V <= 128 ? 2 : 1; }
 int kv4_flash_tiles(int columns, int D, int V, int dt) { return (columns + 64 * kv4_blocks(D, V, dt) - 1) / (64 * kv4_blocks(D, V, dt)); }
 
-template <typename T, int KT, int VH>
-static int kv4_flash_go(const Kv4Attend& p, hipStream_t s) {
-  constexpr int QB = kv4_blocks(32 * KT, 64 * VH, sizeof(T) == 4);
+template <typename T, int KT, int VH, int QB>
+static int kv4_flash_run(const Kv4Attend& p, hipStream_t s) {
   auto kern = kv4_flash_kernel<T, KT, VH, QB>;
   constexpr size_t lds = 2 * Kv4Tile<KT, VH>::kBytes;
   if constexpr (lds > 64 * 1024) {
@@ -404,6 +403,18 @@ static int kv4_flash_go(const Kv4Attend& p, hipStream_t s) {
   if (p.nsplit > 1) hipLaunchKernelGGL((kv4_join_kernel<T, 64 * VH, 64 * QB>), dim3((unsigned)p.items * CB * p.pool.G, 16 * QB), dim3(256), 0, s, p);
   LLJ_CHECK_LAUNCH();
   return 0;
+}
+
+template <typename T, int KT, int VH>
+static int kv4_flash_go(const Kv4Attend& p, hipStream_t s) {
+  constexpr int QB = kv4_blocks(32 * KT, 64 * VH, sizeof(T) == 4);
+  // 128 columns a workgroup share a tile's unpacking; with those of half the CUs or fewer, twice as many of 64 are done sooner (32 heads on 8 of 128, a
+  // prompt of 512 rows 19.4 us, 26.8 in workgroups of 128; of 128 rows 9.2, 13.3; heads of 64, 900 rows 22.5, 30.4)
+  if constexpr (QB == 2) {
+    const long long wgs = (long long)p.items * p.pool.G * ((p.rows * (p.H / p.pool.G) + 127) / 128) * p.nsplit;
+    if (2 * wgs <= 256) return kv4_flash_run<T, KT, VH, 1>(p, s);
+  }
+  return kv4_flash_run<T, KT, VH, QB>(p, s);
 }
 
 template <typename T, int KT>

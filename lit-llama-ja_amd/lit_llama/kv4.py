@@ -19,14 +19,15 @@ from .pages import PAGE_SIZES, ints, on_device
 # K / V heads: 32 ranges 14.2 us, 64 18.0; of 4,000: 16 ranges 10.1, 4 12.7), and 512 workgroups or, of ranges of 1,024 keys, three on a CU (24 sequences
 # of 4,000: 4 ranges 24.5 us, 2 26.4, one 29.5; 32 of 8,000: 3 ranges 49.2, one 54.6; 32 of 2,000: 2 ranges 19.3, one 18.8, 4 21.0). A sequence
 # that is shorter than the table allows takes fewer by itself.
-# Prompt rows: a tile of 64 keys takes TILE us (half as much again with two workgroups on a CU), and ranges a launch of JOIN us that reads what they wrote at
-# PART bytes a us, there and back, and RANGE_STEP us more a range. The sum over n ranges is least at the root of TILE tiles / (what a range costs),
-# measured within a tenth of the best of 12 numbers in 13 of 14 calls (512 rows behind 60,000 tokens: 4 ranges 688 us, one 1,974; 128 rows of 8
-# heads' keys behind 2,048: 7 ranges 28, two 47, one 76; 24 rows of 20 fp32 heads on one behind 9,400: 31 ranges 33, 10 47; 512 rows of a
-# prompt alone: one 25.9, two 28.4).
+# Prompt rows: a tile of 64 keys takes TILE us, half as much again with two workgroups on a CU, 0.7 of it where there are so few that columns are
+# halved (csrc/kv4_flash.hip); ranges take a launch of JOIN us that reads what they wrote at PART bytes a us, there and back, and RANGE_STEP us
+# more a range. Taken is the number with the least sum, of those that fill half the CUs, all, and twice, and the root of TILE tiles / (what a range
+# costs): within 13 % of the best of 12 numbers in 14 calls (512 rows behind 60,000 tokens: 4 ranges 681 us, one 1,445; 128 rows of 8 heads' keys
+# behind 2,048: 4 ranges 24, 16 33, one 55; 24 rows of 20 fp32 heads on one behind 9,400: 31 ranges 33, 10 47; 512 rows of a prompt alone: one
+# 19.4, two 28.8).
 WGS, WGS_LONG = 512, 768
 RANGE, RANGES, RANGE_LONG = 256, 16, 1024
-TILE, JOIN, RANGE_STEP, PART = 2.2, 8.0, 0.2, 4e6
+TILE, JOIN, RANGE_STEP, PART = 2.2, 4.0, 0.2, 4e6
 FEW_COLUMNS = 64  # (row, head) pairs of a K / V head in an item: from more on it is prompt rows (csrc/kv4_attend.hip)
 
 
@@ -159,15 +160,19 @@ def splits(layout: Layout, heads: int, items: int, rows: int, keys: int, dtype: 
     return max(1, min(64, max(min(n, WGS // wgs), min(long, WGS_LONG // wgs)))), items * tiles
 
 
+@lru_cache(4096)
 def _prompt_splits(wgs: int, tiles: int, part: float) -> int:
     """Key ranges of wgs workgroups over so many tiles, whose parts take `part` us a range."""
-    most = min(64, tiles, WGS // wgs)
+    most, each = min(64, tiles, WGS // wgs), RANGE_STEP + wgs * part
     if most < 2:
         return 1
-    each = RANGE_STEP + wgs * part
-    n = max(1, min(most, round((TILE * tiles / each) ** 0.5)))
-    left = -(-tiles // n) * (1.0 if wgs * n <= 256 else 1.5)
-    return n if TILE * (tiles - left) > JOIN + each * n else 1
+
+    def us(n):
+        share = 0.7 if 2 * wgs * n <= 256 else 1.0 if wgs * n <= 256 else 1.5
+        return TILE * share * -(-tiles // n) + (JOIN + each * n if n > 1 else 0.0)
+
+    tried = {1, most, *(max(1, min(most, n)) for n in (round((TILE * tiles / each) ** 0.5), 128 // wgs, 256 // wgs))}
+    return min(sorted(tried), key=us)
 
 
 def item_rows(layout: Layout, heads: int, longest: int) -> int:
