@@ -339,6 +339,25 @@ def test_long_prompt(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,V", [(64, 64), (128, 128), (120, 64), (40, 100)])
+def test_many_prompts(hip, dtype, D, V):
+    """More workgroups than half the CUs, which take 128 columns each where fewer take 64: portions of 17 and 18 rows of 80 sequences, and the same
+    rows in calls of 10 sequences."""
+    g = np.random.default_rng(D)
+    rows = [17 + i % 2 for i in range(80)]
+    c = Case([int(r + n) for r, n in zip(rows, g.integers(0, 190, 80))], rows, 8, 2, D, V, 32, dtype, seed=V)
+    y = c.run(32, gate=True)
+    c.check(y, gate=True)
+    from lit_llama import kv4
+
+    work, pos = c.work(32), ints(c.pos)
+    z = torch.full_like(y, float("nan"))
+    for i in range(0, 80, 10):
+        kv4.attend(c.qd, c.pool, c.lay, c.table, c.slot, pos, work=work[i:i + 10].contiguous(), rows=32, gate=c.gated, out=z)
+    c.check(z, gate=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_that_see_nothing(hip, dtype):
     """pos < 0 (also below -1), slots outside the tables and pages outside the pool: zero rows, with and without ranges and a sink; a gap in
     the middle of a table hides its own tokens only."""
